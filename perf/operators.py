@@ -10,7 +10,8 @@ operations in 32 bits) and as a program calls the framework's kernels:
 
 Quantisation is the same on both sides, step by step in fp32: with
 ``a = max(amax, 2^-100)`` of a block, ``scale = a / 448`` and
-``q = e4m3(x * (448 / a))``.
+``q = e4m3(x * (448 / a))``.  (``448.0 / a`` of a tensor would be a reciprocal
+and a product, two roundings; ``full_like(a, 448) / a`` is the one division.)
 """
 import torch
 
@@ -116,7 +117,7 @@ def _quantize(x, block_rows):
     xp = torch.nn.functional.pad(x.float(), (0, cb * BLOCK - c, 0, rb * block_rows - r))
     xb = xp.view(*lead, rb, block_rows, cb, BLOCK)
     a = xb.abs().amax(dim=(-3, -1), keepdim=True).clamp_min(TINY)
-    q = (xb * (448.0 / a)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(*lead, rb * block_rows, cb * BLOCK)
+    q = (xb * (torch.full_like(a, 448.0) / a)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(*lead, rb * block_rows, cb * BLOCK)
     return q[..., :r, :c], (a / 448.0).view(*lead, rb, cb)
 
 
@@ -393,7 +394,7 @@ def _exact_rows(x):
     for c0 in range(0, c, BLOCK):
         b = x[:, c0:c0 + BLOCK].float()
         a = b.abs().max(dim=1, keepdim=True).values.clamp_min(TINY)
-        q = (b * (448.0 / a)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+        q = (b * (torch.full_like(a, 448.0) / a)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
         out[:, c0:c0 + BLOCK] = q.double() * (a / 448.0).double()
     return out
 
