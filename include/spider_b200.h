@@ -74,6 +74,8 @@ enum {
 enum { SB_ENGINE_AUTO = 0, SB_ENGINE_SIMT = 1, SB_ENGINE_TCGEN05 = 2 };
 /* grouping flags */
 enum { SB_GROUP_POSITIVE_ONLY = 1 };
+/* expert scores of sb_route_experts */
+enum { SB_SCORE_SOFTMAX = 0, SB_SCORE_SIGMOID = 1 };
 
 /* ------------------------------------------------------------------ info */
 /* Bit 0: library built for sm_100a; bit 1: current device is compute capability 10.x. */
@@ -91,6 +93,34 @@ SB_API const char* sb_error_string(int code);
 SB_API int sb_router(const void* h, int act_dtype, int n_tokens, int hidden, const void* router_w,
                      const float* loop_bias_l, int num_experts, int top_k, int32_t* top_idx,
                      float* top_w, float* probs, void* stream);
+
+/* ------------------------------------------------------------------ expert routing from logits
+ * No reference counterpart (the reference's router is sb_router): the routing
+ * of models with more experts, from given logits [n_tokens, num_experts] (dtype
+ * SB_F32 or SB_BF16, row pitch ld elements).
+ *   s = softmax(logits) or sigmoid(logits), c = s + bias (fp32 [E], may be NULL)
+ *   with num_groups > topk_groups: experts [g E/G, (g+1) E/G) are group g, its
+ *   score the sum of its best two c (group_top 2) or its best c (group_top 1);
+ *   only the best topk_groups groups take part
+ *   top_idx = the top_k largest c, descending; top_w = s[top_idx], divided by
+ *   max(their sum, 1e-9) with renormalize, times scale.
+ * Equal choices or group scores: the smaller id first.  Decisions closer than
+ * fp32 resolves are made from fp64 scores.  An expert whose logit or bias is
+ * -inf ranks behind all others and has weight 0; NaN ranks first.
+ * num_experts <= 1024, top_k <= 32, num_groups <= 32 and a divisor of num_experts,
+ * top_k <= topk_groups * num_experts / num_groups.
+ *
+ * sb_route_experts_backward: the gradient of top_w with respect to the logits
+ * with the selection top_idx held fixed, from grad_w [n_tokens, top_k];
+ * grad_logits in the logits' dtype, row pitch ld_grad.  The bias only selects:
+ * it has no gradient (it is passed for its masked experts). */
+SB_API int sb_route_experts(const void* logits, int dtype, int64_t ld, int n_tokens, int num_experts, int top_k,
+                            int score, const float* bias, int num_groups, int topk_groups, int group_top,
+                            int renormalize, float scale, int32_t* top_idx, float* top_w, void* stream);
+SB_API int sb_route_experts_backward(const void* logits, int dtype, int64_t ld, int n_tokens, int num_experts,
+                                     int top_k, int score, const float* bias, int renormalize, float scale,
+                                     const int32_t* top_idx, const float* grad_w, void* grad_logits,
+                                     int64_t ld_grad, void* stream);
 
 /* ------------------------------------------------------------------ grouping
  * Replaces build_dispatch_plan (spider_infer/forge/ep/dispatch.py:56-115) as a
@@ -187,6 +217,105 @@ typedef struct sb_grouped_gemm_args {
 } sb_grouped_gemm_args;
 
 SB_API int sb_grouped_gemm(const sb_grouped_gemm_args* args, void* stream);
+
+/* ------------------------------------------------------------------ block-scaled fp8
+ * e4m3 values with one fp32 scale per block of 128 along the reduction (the
+ * columns) and block_rows rows (1 or 128).  No reference counterpart: its fp8
+ * tensors have one scale per tensor or per row (spider_moe/quant.py:16-69,146-169).
+ *   a = max(amax of |x| over the block, 2^-100); scale = a / 448;
+ *   q = e4m3(x * (448 / a)), each step one fp32 rounding.
+ * x: batch matrices of rows x cols (dtype SB_F32 / SB_BF16), element strides
+ * x_row / x_col / x_batch (any; unit x_col or unit x_row run fast).  q: byte
+ * pitch ldq and batch stride q_batch (multiples of 16, q 16-byte aligned).  scale
+ * element strides scale_row (per block of rows), scale_col, scale_batch.  The
+ * bytes of q past a row's cols are not written.
+ * row_index (block_rows 1 and batch 1 only, may be NULL): row r of q is row
+ * row_index[r] of x, for r < min(rows, *row_count) (device int32, may be NULL). */
+typedef struct sb_fp8_quantize_args {
+  const void* x;
+  int dtype;
+  int block_rows;
+  int batch, rows, cols;
+  int64_t x_row, x_col, x_batch;
+  const int32_t* row_index;
+  const int32_t* row_count;
+  void* q;
+  int64_t ldq, q_batch;
+  float* scale;
+  int64_t scale_row, scale_col, scale_batch;
+} sb_fp8_quantize_args;
+
+SB_API int sb_fp8_quantize_blocks(const sb_fp8_quantize_args* args, void* stream);
+
+/* Product of block-scaled fp8 matrices, plain or grouped by expert, on the
+ * fp8 tensor cores: for row r of group g (rows [offsets[g], offsets[g+1]) of a;
+ * offsets NULL with num_groups 1: all rows)
+ *   acc[r, c] = sum_kb a_scale[r, kb] * b_scale[c / b_block_rows, kb] *
+ *               sum_{k in block kb} a[r, k] * b_g[c, k]
+ * with the inner sums and the running sum in fp32, then the epilogue:
+ *   SB_EPI_LINEAR  out[r, c] = (acc + bias_g[c]) * row_scale[r], fp32 or bf16
+ *   SB_EPI_GELU    out = gelu_erf(acc + bias_g[c])
+ *   SB_EPI_SWIGLU  out = silu(acc_gate + bias_gate_g[c]) * (acc + bias_g[c])
+ * GELU and SwiGLU outputs leave quantised (e4m3 with 1 x 128 blocks, the format
+ * of sb_fp8_quantize_blocks), the operand of the next product.  bias,
+ * bias_gate and row_scale may be NULL.  Output rows outside every group are
+ * not written.  lda, ldb, and for quantised outputs ldo, are byte pitches and
+ * multiples of 16; a, b, b_gate and a quantised out are 16-byte aligned. */
+typedef struct sb_fp8_matmul_args {
+  int epilogue;               /* SB_EPI_LINEAR / GELU / SWIGLU */
+  int out_dtype;              /* LINEAR: SB_F32 / SB_BF16 */
+  int num_groups;             /* <= 1024 */
+  int max_rows;               /* rows of a and out (upper bound of offsets[G]) */
+  int n, k;
+  const void* a;
+  int64_t lda;
+  const float* a_scale;
+  int64_t a_scale_row, a_scale_block;  /* element strides: per row, per block of k */
+  const void* b;              /* [num_groups, n, k], group g starting at row g * b_group_rows */
+  const void* b_gate;         /* SWIGLU: the gate rows, same layout */
+  int64_t ldb, b_group_rows;
+  const float* b_scale;
+  const float* b_gate_scale;
+  int64_t b_scale_row, b_scale_block, b_scale_group;
+  int b_block_rows;           /* 128, or 1 (LINEAR only) */
+  const float* bias;
+  const float* bias_gate;
+  int64_t bias_group;
+  const float* row_scale;
+  const int32_t* offsets;
+  void* out;
+  int64_t ldo;                /* elements (LINEAR) or bytes (quantised) per output row */
+  float* out_scale;
+  int64_t out_scale_row, out_scale_block;
+  int* status;                /* device status word (may be NULL) */
+} sb_fp8_matmul_args;
+
+SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream);
+
+/* The routed experts' FFNs with block-scaled weights: sb_expert_delta for this
+ * format.  Weights [E, ffn, hidden] (up, gate) and [E, hidden, ffn] (down) in
+ * e4m3 with byte pitches ld_in / ld_ffn per row (multiples of 16), scales
+ * contiguous fp32 [E, ceil(rows / 128), ceil(cols / 128)], biases fp32 [E, rows]
+ * or NULL.  Token rows are grouped by expert (repeated ids of a token merged,
+ * weights <= 0 dropped, ids outside [0, E) skipped), quantised, and
+ *   delta[t] = sum over t's experts of w * (down(q(act(up(q(messages[t]))))) + b_down)
+ * in slot order.  messages: row pitch ld elements.  delta: [n_tokens, hidden
+ * rounded up to a multiple of 4] fp32 or bf16 (the extra columns hold no
+ * values).  top_k <= 64.  Workspace status word at offset 0 unless `status` is
+ * given; the workspace needs no initial contents otherwise. */
+typedef struct sb_fp8_experts {
+  int num_experts, hidden, ffn;
+  int activation; /* SB_ACT_GELU / SB_ACT_SWIGLU */
+  int64_t ld_in, ld_ffn;
+  const void* w_up;   const float* s_up;   const float* b_up;
+  const void* w_gate; const float* s_gate; const float* b_gate; /* SwiGLU */
+  const void* w_down; const float* s_down; const float* b_down;
+} sb_fp8_experts;
+
+SB_API size_t sb_fp8_expert_delta_workspace_bytes(const sb_fp8_experts* experts, int n_tokens, int top_k);
+SB_API int sb_fp8_expert_delta(const sb_fp8_experts* experts, const void* messages, int dtype, int64_t ld,
+                               const int32_t* top_idx, const float* top_w, int n_tokens, int top_k, void* delta,
+                               int delta_dtype, int* status, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ edge top-M
  * Replaces spider_edge_topk_f32 (spider_kernels.h:58-60; scalar_phase1_2.cpp:

@@ -29,6 +29,7 @@ SB_ACT_GELU, SB_ACT_SWIGLU = 0, 1
 SB_EPI_LINEAR, SB_EPI_GELU, SB_EPI_SWIGLU, SB_EPI_SWIGLU_IL = 0, 1, 2, 3
 SB_ENGINE_AUTO, SB_ENGINE_SIMT, SB_ENGINE_TCGEN05 = 0, 1, 2
 SB_GROUP_POSITIVE_ONLY = 1
+SB_SCORE_SOFTMAX, SB_SCORE_SIGMOID = 0, 1
 
 ENGINES = {"auto": SB_ENGINE_AUTO, "simt": SB_ENGINE_SIMT, "tcgen05": SB_ENGINE_TCGEN05}
 
@@ -86,12 +87,47 @@ class BlockTaps(C.Structure):
     ]
 
 
+class Fp8QuantizeArgs(C.Structure):
+    _fields_ = [
+        ("x", vp), ("dtype", i32), ("block_rows", i32), ("batch", i32), ("rows", i32), ("cols", i32),
+        ("x_row", i64), ("x_col", i64), ("x_batch", i64), ("row_index", vp), ("row_count", vp),
+        ("q", vp), ("ldq", i64), ("q_batch", i64),
+        ("scale", vp), ("scale_row", i64), ("scale_col", i64), ("scale_batch", i64),
+    ]
+
+
+class Fp8MatmulArgs(C.Structure):
+    _fields_ = [
+        ("epilogue", i32), ("out_dtype", i32), ("num_groups", i32), ("max_rows", i32), ("n", i32), ("k", i32),
+        ("a", vp), ("lda", i64), ("a_scale", vp), ("a_scale_row", i64), ("a_scale_block", i64),
+        ("b", vp), ("b_gate", vp), ("ldb", i64), ("b_group_rows", i64),
+        ("b_scale", vp), ("b_gate_scale", vp), ("b_scale_row", i64), ("b_scale_block", i64), ("b_scale_group", i64),
+        ("b_block_rows", i32), ("bias", vp), ("bias_gate", vp), ("bias_group", i64), ("row_scale", vp),
+        ("offsets", vp), ("out", vp), ("ldo", i64), ("out_scale", vp), ("out_scale_row", i64),
+        ("out_scale_block", i64), ("status", vp),
+    ]
+
+
+class Fp8Experts(C.Structure):
+    _fields_ = [
+        ("num_experts", i32), ("hidden", i32), ("ffn", i32), ("activation", i32), ("ld_in", i64), ("ld_ffn", i64),
+        ("w_up", vp), ("s_up", vp), ("b_up", vp), ("w_gate", vp), ("s_gate", vp), ("b_gate", vp),
+        ("w_down", vp), ("s_down", vp), ("b_down", vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "sb_capabilities": (i32, []),
     "sb_version": (C.c_char_p, []),
     "sb_error_string": (C.c_char_p, [i32]),
     "sb_router": (i32, [vp, i32, i32, i32, vp, vp, i32, i32, vp, vp, vp, vp]),
+    "sb_route_experts": (i32, [vp, i32, i64, i32, i32, i32, i32, vp, i32, i32, i32, i32, f32, vp, vp, vp]),
+    "sb_route_experts_backward": (i32, [vp, i32, i64, i32, i32, i32, i32, vp, i32, f32, vp, vp, vp, i64, vp]),
+    "sb_fp8_quantize_blocks": (i32, [C.POINTER(Fp8QuantizeArgs), vp]),
+    "sb_fp8_matmul": (i32, [C.POINTER(Fp8MatmulArgs), vp]),
+    "sb_fp8_expert_delta_workspace_bytes": (sz, [C.POINTER(Fp8Experts), i32, i32]),
+    "sb_fp8_expert_delta": (i32, [C.POINTER(Fp8Experts), vp, i32, i64, vp, vp, i32, i32, vp, i32, vp, vp, sz, vp]),
     "sb_group_workspace_bytes": (sz, [i32, i32, i32]),
     "sb_group": (i32, [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp]),
     "sb_group_noalloc": (i32, [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]),

@@ -4,6 +4,10 @@
 
 namespace sb {
 
+// 2-D tensor map: inner extent `cols` elements, `rows` rows, row pitch in bytes (sb_gemm_tc.cu).
+bool make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, uint64_t cols, uint64_t rows,
+              uint64_t pitch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw);
+
 // Device-side tile schedule.  Group g owns permuted rows [offsets[g],
 // offsets[g+1]) and ceil(count/BN) column tiles; tiles are numbered group by
 // group.  Executed by one full warp; returns false (uniformly) when `slot` is

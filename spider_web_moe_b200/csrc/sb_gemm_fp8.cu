@@ -1,0 +1,596 @@
+// Products of block-scaled fp8 matrices on the fp8 tensor cores (tcgen05
+// kind::f8f6f4), plain or grouped by expert.
+//
+//   y[r, c] = sum_kb sa[r, kb] sb[c / 128, kb] sum_{k in kb} a[r, k] b[c, k]
+//
+// The scales change every 128 elements of k and are arbitrary fp32 numbers, so
+// the tensor core can only sum one block of 128 at a time: it writes each
+// block's product to one of two TMEM accumulators, and the epilogue warps read
+// it back, scale it and add it to sums in their registers, while the tensor
+// core fills the other accumulator.
+//
+// Orientation: token rows are the MMA's M side (128 per tile, one per TMEM
+// lane), weight rows its N side (2 x 128 per tile).  An epilogue thread then
+// holds one token row, whose scale is one register, and 64 columns of each
+// 128-row weight block, whose scale is another: one multiply-add per element.
+// A SwiGLU tile holds the gate and the up rows of the same 128 features, so
+// the activation and its quantisation for the next product (a 1 x 128 block is
+// the two threads of one token row) need no pass over memory of their own.
+//
+// Warps: 0-7 epilogue (TMEM lane quarter w % 4, columns part w / 4), 8 TMA, 9
+// MMA (+TMEM), 10-11 idle (registers move between whole warpgroups).  Every wait is bounded (sb_common.cuh); loads use no multicast.
+#include "sb_fp8.cuh"
+#include "sb_gemm_common.cuh"
+#include "sb_internal.h"
+
+namespace sb {
+
+struct F8Cfg {
+  static constexpr int kBM = 128, kHalf = 128, kBK = 128;
+  static constexpr int kABytes = kBM * kBK;
+  static constexpr int kHalfBytes = kHalf * kBK;
+  static constexpr int kStageBytes = kABytes + 2 * kHalfBytes;
+  static constexpr int kStages = 4;
+  static constexpr int kAccCols = 2 * kHalf;
+  static constexpr int kTmemCols = 2 * kAccCols;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 384;  // epilogue warpgroups 0-1, TMA / MMA warpgroup 2
+  // Registers per thread at launch (65536 / 384, in steps of 8) and after the
+  // split: an epilogue thread holds 128 sums and 32 values on their way.
+  static constexpr int kRegsLaunch = 168, kRegsEpi = 232, kRegsLoad = 40;
+  static_assert(256 * kRegsEpi + 128 * kRegsLoad <= kThreads * kRegsLaunch, "the split must fit the launch's registers");
+  static constexpr int kSmallRows = 32;  // rows of the box that short tiles load
+  static constexpr int kMaxG = 1024;
+  static constexpr int kOffA = 0;
+  static constexpr int kOffB = kOffA + kStages * kABytes;
+  static constexpr int kOffBar = kOffB + kStages * 2 * kHalfBytes;
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + 4) * 8;
+  static constexpr int kOffMax = kOffMisc + 64;                       // uint32 [2 halves][2 parts][128 rows]
+  static constexpr int kOffBScale = kOffMax + 2 * 2 * kBM * 4;        // float [8 warps][128]
+  static constexpr int kOffPrefix = kOffBScale + kEpiWarps * 128 * 4;  // int [kMaxG + 1]
+  static constexpr int kOffOffsets = kOffPrefix + (kMaxG + 1) * 4;
+  static constexpr int kSmemBytes = kOffOffsets + (kMaxG + 1) * 4 + 1024;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+  static_assert(kTmemCols == 512, "two accumulators of 256 columns");
+};
+
+// Instruction descriptor: e4m3 x e4m3 -> fp32, both K-major, M x N tile.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+SB_DEVINL void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 32 bit, 32 consecutive columns per thread.
+SB_DEVINL void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// One item of the schedule: 128 rows of one group x one column tile.
+struct F8Item {
+  int g, row0, rows, n0;
+};
+SB_DEVINL F8Item f8_item(const int* prefix, const int* s_off, int G, int n_tiles, int tile_cols, int max_rows, int t) {
+  int lo = 0, hi = G - 1;
+  while (lo < hi) {  // largest g with prefix[g] <= t
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  const int local = t - prefix[lo];
+  const int mt = local / n_tiles;
+  F8Item i;
+  i.g = lo;
+  i.row0 = s_off[lo] + mt * F8Cfg::kBM;
+  i.rows = min(min(s_off[lo + 1], max_rows) - i.row0, F8Cfg::kBM);
+  i.n0 = (local - mt * n_tiles) * tile_cols;
+  return i;
+}
+
+// 64 consecutive outputs of one row, `valid` of them in range.
+template <typename T>
+SB_DEVINL void store_row64(T* __restrict__ dst, const float* v, int valid, bool vec) {
+  if (vec && valid >= 64) {
+#pragma unroll
+    for (int i = 0; i < 64; i += 16 / sizeof(T)) {
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 64; ++i)
+    if (i < valid) dst[i] = from_f32<T>(v[i]);
+}
+
+template <int EPI, bool kBRows>
+__global__ void __launch_bounds__(F8Cfg::kThreads, 1)
+f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs,
+               const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmG,
+               const sb_fp8_matmul_args p) {
+  using C = F8Cfg;
+  constexpr int S = C::kStages;
+  constexpr bool kGate = EPI == SB_EPI_SWIGLU;
+  constexpr bool kQuant = EPI != SB_EPI_LINEAR;
+  constexpr int kTileCols = kGate ? C::kHalf : 2 * C::kHalf;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;      // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2]
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
+  int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.num_groups;
+  const int n_tiles = (p.n + kTileCols - 1) / kTileCols;
+  const int nk = (p.k + C::kBK - 1) / C::kBK;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], C::kEpiWarps);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmAs);
+    tma_prefetch_desc(&tmB);
+    if (kGate) tma_prefetch_desc(&tmG);
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {
+    // items per group -> exclusive prefix (warp scan, 32 groups at a time)
+    int seen = 0;
+    for (int base = 0; base < G; base += 32) {
+      const int gi = base + lane;
+      int tiles = 0;
+      if (gi < G) {
+        const int o0 = group_offset(p.offsets, gi, p.max_rows), o1 = group_offset(p.offsets, gi + 1, p.max_rows);
+        s_off[gi] = o0;
+        if (gi == G - 1) s_off[G] = o1;
+        const int lo = min(o0, p.max_rows), hi = min(o1, p.max_rows);
+        tiles = hi > lo ? (hi - lo + C::kBM - 1) / C::kBM * n_tiles : 0;
+      }
+      int incl = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += t;
+      }
+      if (gi < G) prefix[gi] = seen + incl - tiles;
+      seen += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) prefix[G] = seen;
+  }
+  __syncthreads();
+  const int total = prefix[G];
+  if (static_cast<int>(blockIdx.x) >= total) return;  // no item for this CTA
+  if (warp == 9) {
+    tmem_alloc(s_tmem, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLoad));
+    if (warp == 8) {
+      // ---------------------------------------------------------------- TMA
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+          const F8Item w = f8_item(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t);
+          const int brow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
+          const bool small = w.rows <= C::kSmallRows;
+          const bool second = kGate || w.n0 + C::kHalf < p.n;  // the tile's second 128 weight rows exist
+          const uint32_t tx = (small ? C::kSmallRows * C::kBK : C::kABytes) + C::kHalfBytes * (second ? 2 : 1);
+          for (int kk = 0; kk < nk; ++kk, ++it) {
+            const int s = it % S;
+            if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
+            mbar_expect_tx(&full[s], tx);
+            const int k0 = kk * C::kBK;
+            uint8_t* bdst = smem + C::kOffB + s * 2 * C::kHalfBytes;
+            tma_load_2d(bdst, kGate ? &tmG : &tmB, &full[s], k0, brow);
+            if (second) tma_load_2d(bdst + C::kHalfBytes, &tmB, &full[s], k0, kGate ? brow : brow + C::kHalf);
+            tma_load_2d(smem + C::kOffA + s * C::kABytes, small ? &tmAs : &tmA, &full[s], k0, w.row0);
+          }
+        }
+        // every stage released: all copies landed and all commit arrivals done
+        for (int i = it - S > 0 ? it - S : 0; i < it; ++i)
+          if (!mbar_wait(&empty[i % S], (i / S) & 1, p.status, SB_DEVERR_DRAIN)) break;
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // ---------------------------------------------------------------- MMA
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+          const F8Item w = f8_item(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t);
+          const bool second = kGate || w.n0 + C::kHalf < p.n;
+          const uint32_t idesc = idesc_e4m3_f32(C::kBM, second ? 2 * C::kHalf : C::kHalf);
+          for (int kk = 0; kk < nk; ++kk, ++it) {
+            const int s = it % S, buf = it & 1;
+            ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, p.status, SB_DEVERR_EPI_WAIT) &&
+                 mbar_wait(&full[s], (it / S) & 1, p.status, SB_DEVERR_TMA_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a_base = smem_u32(smem + C::kOffA + s * C::kABytes);
+            const uint32_t b_base = smem_u32(smem + C::kOffB + s * 2 * C::kHalfBytes);
+#pragma unroll
+            for (int q = 0; q < C::kBK / 32; ++q)
+              tc_mma_f8(tmem + buf * C::kAccCols, smem_desc_k_sw128(a_base + q * 32), smem_desc_k_sw128(b_base + q * 32),
+                        idesc, q > 0);
+            tc_commit(&empty[s]);
+            tc_commit(&acc_full[buf]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsEpi));
+    const int quarter = warp & 3, part = warp >> 2;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * 64;
+    uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
+    float* s_bs = reinterpret_cast<float*>(smem + C::kOffBScale) + warp * 128;
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const F8Item w = f8_item(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t);
+      const int r = quarter * 32 + lane;          // row of the tile
+      const bool live = r < w.rows;
+      const bool warp_live = quarter * 32 < w.rows;
+      const int64_t row = w.row0 + r;
+      const float* sa_ptr = p.a_scale + row * p.a_scale_row;
+      const float* sb0 = (kGate ? p.b_gate_scale : p.b_scale) + w.g * p.b_scale_group;
+      const float* sb1 = p.b_scale + w.g * p.b_scale_group;
+      if (!kBRows) {
+        sb0 += (w.n0 / 128) * p.b_scale_row;
+        sb1 += (w.n0 / 128 + (kGate ? 0 : 1)) * p.b_scale_row;
+      }
+      const bool second = kGate || w.n0 + C::kHalf < p.n;
+      // kBRows: lane i stages the scales of four of the warp's 128 columns
+      const int bcol = w.n0 + (lane >> 4) * C::kHalf + part * 64 + (lane & 15) * 4;
+      float acc[2][64];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 64; ++i) acc[h][i] = 0.f;
+      for (int kk = 0; kk < nk; ++kk, ++it) {
+        const int buf = it & 1;
+        const float sa = live ? sa_ptr[kk * p.a_scale_block] : 0.f;
+        float s0 = 0.f, s1 = 0.f;
+        if (kBRows) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s_bs[lane * 4 + j] = bcol + j < p.n ? sb1[(bcol + j) * p.b_scale_row + kk * p.b_scale_block] : 0.f;
+          __syncwarp();
+        } else {
+          s0 = sa * sb0[kk * p.b_scale_block];
+          if (second) s1 = sa * sb1[kk * p.b_scale_block];
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_live) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !second) break;
+            const float s = h ? s1 : s0;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+              float v[32];
+              tmem_ld32(lane_addr + buf * C::kAccCols + h * C::kHalf + c, v);
+              if (kBRows) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[h][c + i] = fmaf(v[i] * s_bs[h * 64 + c + i], sa, acc[h][c + i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[h][c + i] = fmaf(v[i], s, acc[h][c + i]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      }
+      if constexpr (!kQuant) {
+        if (!ok || !warp_live) continue;
+        const float rs = live && p.row_scale ? p.row_scale[row] : 1.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c0 = w.n0 + h * C::kHalf + part * 64;
+          const int valid = p.n - c0;
+          if (valid <= 0) continue;
+          if (p.bias) {
+            const float* bias = p.bias + w.g * p.bias_group + c0;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[h][i] += i < valid ? bias[i] : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 64; ++i) acc[h][i] *= rs;
+          if (!live) continue;
+          if (p.out_dtype == SB_F32) {
+            float* dst = static_cast<float*>(p.out) + row * p.ldo + c0;
+            store_row64(dst, acc[h], valid, reinterpret_cast<uintptr_t>(dst) % 16 == 0);
+          } else {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + c0;
+            store_row64(dst, acc[h], valid, reinterpret_cast<uintptr_t>(dst) % 16 == 0);
+          }
+        }
+      } else {
+        // activation, then one 1 x 128 block per row (SwiGLU) or two (GELU),
+        // each held by this thread and the other part's thread of the same row
+        constexpr int kBlocks = kGate ? 1 : 2;
+        uint32_t amax[kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          const int c0 = w.n0 + b * C::kHalf + part * 64;
+          const int valid = p.n - c0;
+          const float* bias = p.bias ? p.bias + w.g * p.bias_group + c0 : nullptr;
+          const float* bgate = kGate && p.bias_gate ? p.bias_gate + w.g * p.bias_group + c0 : nullptr;
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            float y;
+            if (kGate) {
+              const float up = acc[1][i] + (bias && i < valid ? bias[i] : 0.f);
+              y = silu(acc[0][i] + (bgate && i < valid ? bgate[i] : 0.f)) * up;
+            } else {
+              y = gelu_erf(acc[b][i] + (bias && i < valid ? bias[i] : 0.f));
+            }
+            y = i < valid ? y : 0.f;
+            acc[b][i] = y;
+            m = max(m, abs_bits(y));
+          }
+          amax[b] = m;
+          s_max[(b * 2 + part) * C::kBM + r] = m;
+        }
+        ok = named_bar_and(1 + quarter, 64, ok);
+        if (live && ok) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const int c0 = w.n0 + b * C::kHalf + part * 64;
+            if (w.n0 + b * C::kHalf >= p.n) continue;
+            const Fp8Scale s = fp8_scale(max(amax[b], s_max[(b * 2 + (part ^ 1)) * C::kBM + r]));
+            if (part == 0)
+              p.out_scale[row * p.out_scale_row + (w.n0 / 128 + b) * p.out_scale_block] = s.scale;
+            uint8_t* dst = static_cast<uint8_t*>(p.out) + row * p.ldo + c0;
+#pragma unroll
+            for (int i = 0; i < 64; i += 16) {
+              uint32_t q[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                q[k] = fp8_pack4(acc[b][i + 4 * k] * s.inv, acc[b][i + 4 * k + 1] * s.inv,
+                                 acc[b][i + 4 * k + 2] * s.inv, acc[b][i + 4 * k + 3] * s.inv);
+              if (c0 + i + 16 <= p.n) {
+                *reinterpret_cast<uint4*>(dst + i) = make_uint4(q[0], q[1], q[2], q[3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  if (c0 + i + j < p.n) dst[i + j] = static_cast<uint8_t>(q[j >> 2] >> (8 * (j & 3)));
+              }
+            }
+          }
+        }
+        named_bar_sync(1 + quarter, 64);  // s_max is free for the next item
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+static bool f8_map(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int64_t pitch, int box_rows) {
+  return make_map(m, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, k, rows, pitch, F8Cfg::kBK, box_rows,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int EPI, bool kBRows>
+static int launch_f8(const sb_fp8_matmul_args& a, cudaStream_t st) {
+  using C = F8Cfg;
+  auto kern = f8_gemm_kernel<EPI, kBRows>;
+  static int configured_device = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_device != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    if (e != cudaSuccess) return cuda_status(e);
+    configured_device = dev;
+  }
+  constexpr int kTileCols = EPI == SB_EPI_SWIGLU ? C::kHalf : 2 * C::kHalf;
+  const int64_t b_rows = (a.num_groups - 1) * a.b_group_rows + a.n;
+  CUtensorMap ma, mas, mb, mg;
+  if (!f8_map(&ma, a.a, a.k, a.max_rows, a.lda, C::kBM) || !f8_map(&mas, a.a, a.k, a.max_rows, a.lda, C::kSmallRows) ||
+      !f8_map(&mb, a.b, a.k, b_rows, a.ldb, C::kHalf))
+    return SB_ERR_UNSUPPORTED;
+  mg = mb;
+  if (EPI == SB_EPI_SWIGLU && !f8_map(&mg, a.b_gate, a.k, b_rows, a.ldb, C::kHalf)) return SB_ERR_UNSUPPORTED;
+  const int64_t n_tiles = (a.n + kTileCols - 1) / kTileCols;
+  const int64_t row_tiles = (a.max_rows + C::kBM - 1) / C::kBM + (a.offsets ? a.num_groups : 0);
+  if (n_tiles * row_tiles > 0x7fffffff) return SB_ERR_UNSUPPORTED;
+  const int64_t sms = current_sm_count();
+  const int grid = static_cast<int>(n_tiles * row_tiles < sms ? n_tiles * row_tiles : sms);
+  return launch(kern, dim3(grid), dim3(C::kThreads), C::kSmemBytes, st, ma, mas, mb, mg, a);
+}
+
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream) {
+  if (!args) return SB_ERR_ARG;
+  const sb_fp8_matmul_args& a = *args;
+  const bool quant = a.epilogue == SB_EPI_GELU || a.epilogue == SB_EPI_SWIGLU;
+  if ((!quant && a.epilogue != SB_EPI_LINEAR) || (!quant && a.out_dtype != SB_F32 && a.out_dtype != SB_BF16) ||
+      a.num_groups < 1 || a.num_groups > F8Cfg::kMaxG || (!a.offsets && a.num_groups != 1) || a.max_rows < 0 ||
+      a.n < 1 || a.k < 1 || (a.b_block_rows != 128 && a.b_block_rows != 1) || (quant && a.b_block_rows != 128) ||
+      a.lda < a.k || a.lda % 16 || a.ldb < a.k || a.ldb % 16 || (a.num_groups > 1 && a.b_group_rows < a.n) ||
+      a.ldo < a.n || (quant && a.ldo % 16))
+    return SB_ERR_ARG;
+  if (a.max_rows == 0) return SB_OK;
+  auto aligned = [](const void* p) { return p && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  if (!aligned(a.a) || !aligned(a.b) || !a.a_scale || !a.b_scale || !a.out || (quant && (!aligned(a.out) || !a.out_scale)) ||
+      (a.epilogue == SB_EPI_SWIGLU && (!aligned(a.b_gate) || !a.b_gate_scale)))
+    return SB_ERR_ARG;
+  if ((a.num_groups - 1) * a.b_group_rows + a.n > 0x7fffffff) return SB_ERR_UNSUPPORTED;  // TMA row coordinates
+  if (current_cc_major() != 10) return SB_ERR_NO_DEVICE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a.epilogue == SB_EPI_SWIGLU) return launch_f8<SB_EPI_SWIGLU, false>(a, st);
+  if (a.epilogue == SB_EPI_GELU) return launch_f8<SB_EPI_GELU, false>(a, st);
+  return a.b_block_rows == 1 ? launch_f8<SB_EPI_LINEAR, true>(a, st) : launch_f8<SB_EPI_LINEAR, false>(a, st);
+}
+
+// ------------------------------------------------------------------ expert delta
+namespace sb {
+
+struct F8DeltaBuffers {
+  int32_t *off, *row, *slot, *inv;
+  float* w;
+  void* group_ws;
+  size_t group_ws_bytes;
+  uint8_t *xq, *act;
+  float *xs, *as, *y;
+  int* status;
+};
+
+static bool f8_experts_ok(const sb_fp8_experts* x) {
+  return x && x->num_experts >= 1 && x->num_experts <= F8Cfg::kMaxG && x->hidden >= 1 && x->ffn >= 1 &&
+         (x->activation == SB_ACT_GELU || x->activation == SB_ACT_SWIGLU) && x->ld_in % 16 == 0 && x->ld_in >= x->hidden &&
+         x->ld_ffn % 16 == 0 && x->ld_ffn >= x->ffn;
+}
+
+// Carves the scratch of one call; returns the bytes it takes.
+static size_t f8_carve(const sb_fp8_experts& x, int n, int k, void* ws, size_t bytes, F8DeltaBuffers* b) {
+  Carver c(ws, bytes);
+  const size_t pairs = static_cast<size_t>(n) * k, pr = align_up(pairs, 4);
+  b->status = c.take<int>(kStatusBytes / sizeof(int));
+  b->off = c.take<int32_t>(x.num_experts + 1);
+  b->row = c.take<int32_t>(pairs);
+  b->slot = c.take<int32_t>(pairs);
+  b->inv = c.take<int32_t>(pairs);
+  b->w = c.take<float>(pairs);
+  b->group_ws_bytes = sb_group_workspace_bytes(n, k, x.num_experts);
+  b->group_ws = c.take<uint8_t>(b->group_ws_bytes);
+  b->xq = c.take<uint8_t>(pairs * align_up(x.hidden, 16));
+  b->xs = c.take<float>(pr * ((x.hidden + 127) / 128));
+  b->act = c.take<uint8_t>(pairs * align_up(x.ffn, 16));
+  b->as = c.take<float>(pr * ((x.ffn + 127) / 128));
+  b->y = c.take<float>(pairs * align_up(x.hidden, 4));
+  return c.overflow ? static_cast<size_t>(-1) : align_up(c.used, 256);
+}
+
+}  // namespace sb
+
+extern "C" SB_API size_t sb_fp8_expert_delta_workspace_bytes(const sb_fp8_experts* experts, int n_tokens, int top_k) {
+  if (!f8_experts_ok(experts) || n_tokens < 0 || top_k < 1 || top_k > 64 ||
+      static_cast<int64_t>(n_tokens) * top_k > 0x7fffffff)
+    return 0;
+  F8DeltaBuffers b;
+  return f8_carve(*experts, n_tokens > 0 ? n_tokens : 1, top_k, nullptr, ~size_t(0) >> 1, &b);
+}
+
+extern "C" SB_API int sb_fp8_expert_delta(const sb_fp8_experts* experts, const void* messages, int dtype, int64_t ld,
+                                          const int32_t* top_idx, const float* top_w, int n_tokens, int top_k,
+                                          void* delta, int delta_dtype, int* status, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  if (!f8_experts_ok(experts) || (dtype != SB_F32 && dtype != SB_BF16) ||
+      (delta_dtype != SB_F32 && delta_dtype != SB_BF16) || n_tokens < 0 || top_k < 1 || top_k > 64 ||
+      static_cast<int64_t>(n_tokens) * top_k > 0x7fffffff || ld < experts->hidden)
+    return SB_ERR_ARG;
+  if (n_tokens == 0) return SB_OK;
+  const sb_fp8_experts& x = *experts;
+  const bool swiglu = x.activation == SB_ACT_SWIGLU;
+  if (!messages || !top_idx || !top_w || !delta || !x.w_up || !x.s_up || !x.w_down || !x.s_down ||
+      (swiglu && (!x.w_gate || !x.s_gate)))
+    return SB_ERR_ARG;
+  F8DeltaBuffers b;
+  const size_t need = f8_carve(x, n_tokens, top_k, workspace, workspace_bytes, &b);
+  if (!workspace || need == static_cast<size_t>(-1) || need > workspace_bytes) return SB_ERR_WORKSPACE;
+  const int N = n_tokens, E = x.num_experts, H = x.hidden, U = x.ffn, P = N * top_k;
+  const int64_t pr = align_up(P, 4);
+  const int hb = (H + 127) / 128, ub = (U + 127) / 128;
+  if (!status) status = b.status;
+#define SB_TRY(e) do { const int rc = (e); if (rc) return rc; } while (0)
+  SB_TRY(sb_group(top_idx, top_w, N, top_k, E, SB_GROUP_POSITIVE_ONLY, b.off, b.row, b.slot, b.w, b.inv, b.group_ws,
+                  b.group_ws_bytes, stream));
+  sb_fp8_quantize_args q = {};
+  q.x = messages; q.dtype = dtype; q.block_rows = 1; q.batch = 1; q.rows = P; q.cols = H;
+  q.x_row = ld; q.x_col = 1; q.row_index = b.row; q.row_count = b.off + E;
+  q.q = b.xq; q.ldq = align_up(H, 16); q.scale = b.xs; q.scale_row = 1; q.scale_col = pr;
+  SB_TRY(sb_fp8_quantize_blocks(&q, stream));
+  sb_fp8_matmul_args a = {};
+  a.epilogue = swiglu ? SB_EPI_SWIGLU : SB_EPI_GELU;
+  a.num_groups = E; a.max_rows = P; a.n = U; a.k = H; a.offsets = b.off; a.status = status; a.b_block_rows = 128;
+  a.a = b.xq; a.lda = q.ldq; a.a_scale = b.xs; a.a_scale_row = 1; a.a_scale_block = pr;
+  a.b = x.w_up; a.b_gate = x.w_gate; a.ldb = x.ld_in; a.b_group_rows = U;
+  a.b_scale = x.s_up; a.b_gate_scale = x.s_gate;
+  a.b_scale_row = hb; a.b_scale_block = 1; a.b_scale_group = static_cast<int64_t>(ub) * hb;
+  a.bias = x.b_up; a.bias_gate = x.b_gate; a.bias_group = U;
+  a.out = b.act; a.ldo = align_up(U, 16); a.out_scale = b.as; a.out_scale_row = 1; a.out_scale_block = pr;
+  SB_TRY(sb_fp8_matmul(&a, stream));
+  sb_fp8_matmul_args d = {};
+  d.epilogue = SB_EPI_LINEAR; d.out_dtype = SB_F32;
+  d.num_groups = E; d.max_rows = P; d.n = H; d.k = U; d.offsets = b.off; d.status = status; d.b_block_rows = 128;
+  d.a = b.act; d.lda = a.ldo; d.a_scale = b.as; d.a_scale_row = 1; d.a_scale_block = pr;
+  d.b = x.w_down; d.ldb = x.ld_ffn; d.b_group_rows = H;
+  d.b_scale = x.s_down; d.b_scale_row = ub; d.b_scale_block = 1; d.b_scale_group = static_cast<int64_t>(hb) * ub;
+  d.bias = x.b_down; d.bias_group = H; d.row_scale = b.w;
+  d.out = b.y; d.ldo = align_up(H, 4);
+  SB_TRY(sb_fp8_matmul(&d, stream));
+  const int cols = static_cast<int>(align_up(H, 4));
+  SB_TRY(sb_combine_rows(b.y, cols, 1, 0, b.inv, top_k, N, cols,
+                         delta_dtype == SB_F32 ? static_cast<float*>(delta) : nullptr, nullptr, 0,
+                         delta_dtype == SB_F32 ? nullptr : delta, SB_BF16, stream));
+#undef SB_TRY
+  return SB_OK;
+}

@@ -1784,7 +1784,7 @@ static EncodeTiledFn encode_fn() {
 }
 
 // 2-D tensor map: inner extent `cols` elements, `rows` rows, row pitch in bytes.
-static bool make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, uint64_t cols, uint64_t rows,
+bool make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, uint64_t cols, uint64_t rows,
                      uint64_t pitch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
