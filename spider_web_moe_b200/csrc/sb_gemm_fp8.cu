@@ -9,49 +9,72 @@
 // it back, scale it and add it to sums in their registers, while the tensor
 // core fills the other accumulator.
 //
-// Orientation: token rows are the MMA's M side (128 per tile, one per TMEM
-// lane), weight rows its N side (2 x 128 per tile).  An epilogue thread then
-// holds one token row, whose scale is one register, and 64 columns of each
-// 128-row weight block, whose scale is another: one multiply-add per element.
-// A SwiGLU tile holds the gate and the up rows of the same 128 features, so
-// the activation and its quantisation for the next product (a 1 x 128 block is
-// the two threads of one token row) need no pass over memory of their own.
+// Orientation: token rows are the MMA's M side (one per TMEM lane), weight rows
+// its N side (2 x 128 per tile).  An epilogue thread then holds one token row,
+// whose scale is one register, and 32 columns of each 128-row weight block,
+// whose scale is another: one multiply-add per element, two at a time
+// (fma.rn.f32x2).  A SwiGLU tile holds the gate and the up rows of the same 128
+// features, so the activation and its quantisation for the next product (a
+// 1 x 128 block is the four threads of one token row) need no pass over memory
+// of their own.
 //
-// Warps: 0-7 epilogue (TMEM lane quarter w % 4, columns part w / 4), 8 TMA, 9
-// MMA (+TMEM), 10-11 idle (registers move between whole warpgroups).  Every wait is bounded (sb_common.cuh); loads use no multicast.
+// Two schedules.  One CTA per tile of 128 rows (decode batches, small groups);
+// CTA pairs for tiles of 256 rows (cta_group::2): each CTA loads its own 128
+// rows of a and half of the weight rows, which halves the weight traffic into
+// shared memory, the limit of the one-CTA tile.
+//
+// Warps: 0-15 epilogue (TMEM lane quarter w % 4, columns part w / 4), 16 TMA, 17
+// MMA (+TMEM).  Every wait is bounded (sb_common.cuh); loads use no multicast.
 #include "sb_fp8.cuh"
 #include "sb_gemm_common.cuh"
 #include "sb_internal.h"
 
+#ifndef F8_PARTS
+#define F8_PARTS 2
+#define F8_CHUNK 32
+#endif
 namespace sb {
 
+constexpr int kF8MaxG = 1024;
+
+template <bool kPair>
 struct F8Cfg {
-  static constexpr int kBM = 128, kHalf = 128, kBK = 128;
+  static constexpr int kBM = 128;                      // rows per CTA
+  static constexpr int kItemRows = kPair ? 256 : 128;  // rows per item
+  static constexpr int kHalf = 128, kBK = 128;
   static constexpr int kABytes = kBM * kBK;
   static constexpr int kHalfBytes = kHalf * kBK;
-  static constexpr int kStageBytes = kABytes + 2 * kHalfBytes;
+  static constexpr int kBBytes = kHalfBytes * (kPair ? 1 : 2);  // weight rows this CTA holds
+  static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = 4;
   static constexpr int kAccCols = 2 * kHalf;
   static constexpr int kTmemCols = 2 * kAccCols;
-  static constexpr int kEpiWarps = 8;
-  static constexpr int kThreads = 384;  // epilogue warpgroups 0-1, TMA / MMA warpgroup 2
-  // Registers per thread at launch (65536 / 384, in steps of 8) and after the
-  // split: an epilogue thread holds 128 sums and 32 values on their way.
-  static constexpr int kRegsLaunch = 168, kRegsEpi = 232, kRegsLoad = 40;
-  static_assert(256 * kRegsEpi + 128 * kRegsLoad <= kThreads * kRegsLaunch, "the split must fit the launch's registers");
-  static constexpr int kSmallRows = 32;  // rows of the box that short tiles load
-  static constexpr int kMaxG = 1024;
+  static constexpr int kParts = F8_PARTS;                     // epilogue warps per TMEM lane quarter
+  static constexpr int kCols = kHalf / kParts;         // columns of each half per epilogue thread
+  static constexpr int kEpiWarps = 4 * kParts;
+  static constexpr int kChunk = F8_CHUNK;              // columns per TMEM load
+  static constexpr int kThreads = (kEpiWarps + 4) * 32;  // whole warpgroups: registers move between them
+  // Registers per thread at launch (65536 / kThreads, in steps of 8) and after
+  // the split.
+  static constexpr int kRegsLaunch = kParts == 2 ? 168 : 96;
+  static constexpr int kRegsEpi = kParts == 2 ? 224 : 104, kRegsLoad = kParts == 2 ? 56 : 64;
+  static_assert(kEpiWarps * 32 * kRegsEpi + 128 * kRegsLoad <= kThreads * kRegsLaunch, "the split must fit the launch's registers");
+  static constexpr int kSmallRows = 32;                // rows of the box that short tiles load
   static constexpr int kOffA = 0;
   static constexpr int kOffB = kOffA + kStages * kABytes;
-  static constexpr int kOffBar = kOffB + kStages * 2 * kHalfBytes;
+  // output staging of the pair schedule: two boxes of 32 rows x 128 bytes per epilogue warp
+  static constexpr int kBoxBytes = 32 * 128;
+  static constexpr int kOffOut = kOffB + kStages * kBBytes;
+  static constexpr int kOffBar = kOffOut + (kPair ? kEpiWarps * 2 * kBoxBytes : 0);
   static constexpr int kOffMisc = kOffBar + (2 * kStages + 4) * 8;
-  static constexpr int kOffMax = kOffMisc + 64;                       // uint32 [2 halves][2 parts][128 rows]
-  static constexpr int kOffBScale = kOffMax + 2 * 2 * kBM * 4;        // float [8 warps][128]
-  static constexpr int kOffPrefix = kOffBScale + kEpiWarps * 128 * 4;  // int [kMaxG + 1]
-  static constexpr int kOffOffsets = kOffPrefix + (kMaxG + 1) * 4;
-  static constexpr int kSmemBytes = kOffOffsets + (kMaxG + 1) * 4 + 1024;
+  static constexpr int kOffMax = kOffMisc + 64;                            // uint32 [2 blocks][kParts][128 rows]
+  static constexpr int kOffBScale = kOffMax + 2 * kParts * kBM * 4;        // float [warps][2][kCols]
+  static constexpr int kOffPrefix = kOffBScale + kEpiWarps * 2 * kCols * 4;  // int [kF8MaxG + 1]
+  static constexpr int kOffOffsets = kOffPrefix + (kF8MaxG + 1) * 4;
+  static constexpr int kSmemBytes = kOffOffsets + (kF8MaxG + 1) * 4 + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(kTmemCols == 512, "two accumulators of 256 columns");
+  static_assert(kOffBScale % 16 == 0, "float2 reads");
 };
 
 // Instruction descriptor: e4m3 x e4m3 -> fp32, both K-major, M x N tile.
@@ -59,38 +82,87 @@ __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+template <bool kPair>
 SB_DEVINL void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
-// 32 lanes x 32 bit, 32 consecutive columns per thread.
-SB_DEVINL void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
+// 32 lanes x 32 bit, kN consecutive columns per thread, in pairs of columns.
+template <int kN>
+SB_DEVINL void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[kN / 2]) {
+  static_assert(kN == 16 || kN == 32, "x16 or x32 loads");
+  uint32_t r[kN];
+  if constexpr (kN == 32)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < kN / 2; ++i) asm("mov.b64 %0, {%1, %2};" : "=l"(v[i]) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+}
+// Arrive on the leader's accumulator barrier.  What it hands over is TMEM, ordered
+// by the tcgen05 fences on both sides, so the default CTA-scope release does: a
+// cluster-scope one waits for every outstanding access of the thread, once per
+// block of k (measured on 16384 x 4096 x 8192: 1190 us with it).
+SB_DEVINL void mbar_arrive_leader(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+SB_DEVINL uint64_t pair_of(float x) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+  return r;
+}
+SB_DEVINL void fma_pair(uint64_t& acc, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+SB_DEVINL uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// One item of the schedule: 128 rows of one group x one column tile.
+// One item of the schedule: the rows of this CTA of one row tile of one group,
+// and a column tile.
 struct F8Item {
-  int g, row0, rows, n0;
+  int g;
+  int row0;    // first row of this CTA
+  int rows;    // valid rows of this CTA (may be <= 0 in a pair)
+  int peer;    // valid rows of the item's other CTA (pair only)
+  int n0;
 };
-SB_DEVINL F8Item f8_item(const int* prefix, const int* s_off, int G, int n_tiles, int tile_cols, int max_rows, int t) {
+template <bool kPair>
+SB_DEVINL F8Item f8_item(const int* prefix, const int* s_off, int G, int n_tiles, int tile_cols, int max_rows, int t,
+                         int rank) {
+  using C = F8Cfg<kPair>;
   int lo = 0, hi = G - 1;
   while (lo < hi) {  // largest g with prefix[g] <= t
     const int mid = (lo + hi + 1) >> 1;
@@ -98,60 +170,71 @@ SB_DEVINL F8Item f8_item(const int* prefix, const int* s_off, int G, int n_tiles
   }
   const int local = t - prefix[lo];
   const int mt = local / n_tiles;
+  const int tile_row0 = s_off[lo] + mt * C::kItemRows;
+  const int left = min(s_off[lo + 1], max_rows) - tile_row0;
   F8Item i;
   i.g = lo;
-  i.row0 = s_off[lo] + mt * F8Cfg::kBM;
-  i.rows = min(min(s_off[lo + 1], max_rows) - i.row0, F8Cfg::kBM);
+  i.row0 = tile_row0 + rank * C::kBM;
+  i.rows = min(left - rank * C::kBM, C::kBM);
+  i.peer = kPair ? min(left - (1 - rank) * C::kBM, C::kBM) : 0;
   i.n0 = (local - mt * n_tiles) * tile_cols;
   return i;
 }
 
-// 64 consecutive outputs of one row, `valid` of them in range.
-template <typename T>
-SB_DEVINL void store_row64(T* __restrict__ dst, const float* v, int valid, bool vec) {
-  if (vec && valid >= 64) {
+SB_DEVINL uint32_t bf16_pair(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 16-byte chunk of a row of a staging box (rows of 128 bytes, 128-byte swizzle).
+SB_DEVINL uint4* box_chunk(uint8_t* box, int row, int chunk) {
+  return reinterpret_cast<uint4*>(box + row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+// kN consecutive outputs of one row, `valid` of them in range.
+template <typename T, int kN>
+SB_DEVINL void store_row(T* __restrict__ dst, const float (&v)[kN], int valid, bool vec) {
+  if (vec && valid >= kN) {
 #pragma unroll
-    for (int i = 0; i < 64; i += 16 / sizeof(T)) {
+    for (int i = 0; i < kN; i += 16 / sizeof(T)) {
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
-          w[k] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + i) = make_uint4(bf16_pair(v[i], v[i + 1]), bf16_pair(v[i + 2], v[i + 3]),
+                                                        bf16_pair(v[i + 4], v[i + 5]), bf16_pair(v[i + 6], v[i + 7]));
       }
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 64; ++i)
+  for (int i = 0; i < kN; ++i)
     if (i < valid) dst[i] = from_f32<T>(v[i]);
 }
 
-template <int EPI, bool kBRows>
-__global__ void __launch_bounds__(F8Cfg::kThreads, 1)
+template <int EPI, bool kBRows, bool kPair>
+__global__ void __launch_bounds__(F8Cfg<kPair>::kThreads, 1)
 f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs,
                const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmG,
-               const sb_fp8_matmul_args p) {
-  using C = F8Cfg;
+               const __grid_constant__ CUtensorMap tmO, const sb_fp8_matmul_args p, const int tma_out) {
+  using C = F8Cfg<kPair>;
   constexpr int S = C::kStages;
   constexpr bool kGate = EPI == SB_EPI_SWIGLU;
   constexpr bool kQuant = EPI != SB_EPI_LINEAR;
   constexpr int kTileCols = kGate ? C::kHalf : 2 * C::kHalf;
+  constexpr int kTmaWarp = C::kEpiWarps, kMmaWarp = C::kEpiWarps + 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // a pair uses the leader's
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;      // [2]
-  uint64_t* acc_empty = acc_full + 2;  // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2], a pair uses the leader's
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int stride = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
   const int G = p.num_groups;
   const int n_tiles = (p.n + kTileCols - 1) / kTileCols;
   const int nk = (p.k + C::kBK - 1) / C::kBK;
@@ -162,11 +245,11 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], C::kEpiWarps);
+      mbar_init(&acc_empty[b], C::kEpiWarps * (kPair ? 2 : 1));
     }
     fence_barrier_init();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kTmaWarp && lane == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmAs);
     tma_prefetch_desc(&tmB);
@@ -185,7 +268,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         s_off[gi] = o0;
         if (gi == G - 1) s_off[G] = o1;
         const int lo = min(o0, p.max_rows), hi = min(o1, p.max_rows);
-        tiles = hi > lo ? (hi - lo + C::kBM - 1) / C::kBM * n_tiles : 0;
+        tiles = hi > lo ? (hi - lo + C::kItemRows - 1) / C::kItemRows * n_tiles : 0;
       }
       int incl = tiles;
 #pragma unroll
@@ -198,89 +281,122 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     }
     if (lane == 0) prefix[G] = seen;
   }
-  __syncthreads();
+  if constexpr (kPair) {
+    __syncwarp();
+    cluster_sync();  // both CTAs' barriers exist before either signals the other
+  } else {
+    __syncthreads();
+  }
   const int total = prefix[G];
-  if (static_cast<int>(blockIdx.x) >= total) return;  // no item for this CTA
-  if (warp == 9) {
-    tmem_alloc(s_tmem, C::kTmemCols);
-    tmem_relinquish();
+  if (first >= total) return;  // no item for this CTA (or for either of the pair)
+  if (warp == kMmaWarp) {
+    if constexpr (kPair) {
+      tmem_alloc_pair(s_tmem, C::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(s_tmem, C::kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  if (warp >= 8) {
+  if (warp >= C::kEpiWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLoad));
-    if (warp == 8) {
-      // ---------------------------------------------------------------- TMA
-      if (lane == 0) {
-        int it = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-          const F8Item w = f8_item(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t);
-          const int brow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
-          const bool small = w.rows <= C::kSmallRows;
-          const bool second = kGate || w.n0 + C::kHalf < p.n;  // the tile's second 128 weight rows exist
-          const uint32_t tx = (small ? C::kSmallRows * C::kBK : C::kABytes) + C::kHalfBytes * (second ? 2 : 1);
-          for (int kk = 0; kk < nk; ++kk, ++it) {
-            const int s = it % S;
-            if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
+    if (warp == kTmaWarp) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += stride) {
+        const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
+        const bool second = kGate || w.n0 + C::kHalf < p.n;  // the tile's second 128 weight rows exist
+        const int brow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
+        auto a_bytes = [&](int rows) {  // a CTA without rows loads none: its lanes are never read
+          return static_cast<uint32_t>(rows <= 0 ? 0 : (rows <= C::kSmallRows ? C::kSmallRows * C::kBK : C::kABytes));
+        };
+        const uint32_t tx = kPair ? a_bytes(w.rows) + a_bytes(w.peer) + 2 * C::kHalfBytes
+                                  : a_bytes(w.rows) + C::kHalfBytes * (second ? 2 : 1);
+        const CUtensorMap* map_a = w.rows <= C::kSmallRows ? &tmAs : &tmA;
+        for (int kk = 0; kk < nk; ++kk, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
+          const int k0 = kk * C::kBK;
+          uint8_t* adst = smem + C::kOffA + s * C::kABytes;
+          uint8_t* bdst = smem + C::kOffB + s * C::kBBytes;
+          if constexpr (kPair) {
+            // both CTAs' bytes count on the leader's barrier.  The MMA takes the
+            // first half of its N columns from CTA 0, the second from CTA 1.
+            if (rank == 0) mbar_expect_tx(&full[s], tx);
+            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+            tma_load_2d_pair(bdst, kGate && rank == 0 ? &tmG : &tmB, bar, k0,
+                             kGate || rank == 0 ? brow : brow + (second ? C::kHalf : C::kHalf / 2));
+            if (w.rows > 0) tma_load_2d_pair(adst, map_a, bar, k0, w.row0);
+          } else {
             mbar_expect_tx(&full[s], tx);
-            const int k0 = kk * C::kBK;
-            uint8_t* bdst = smem + C::kOffB + s * 2 * C::kHalfBytes;
             tma_load_2d(bdst, kGate ? &tmG : &tmB, &full[s], k0, brow);
             if (second) tma_load_2d(bdst + C::kHalfBytes, &tmB, &full[s], k0, kGate ? brow : brow + C::kHalf);
-            tma_load_2d(smem + C::kOffA + s * C::kABytes, small ? &tmAs : &tmA, &full[s], k0, w.row0);
+            tma_load_2d(adst, map_a, &full[s], k0, w.row0);
           }
         }
-        // every stage released: all copies landed and all commit arrivals done
-        for (int i = it - S > 0 ? it - S : 0; i < it; ++i)
-          if (!mbar_wait(&empty[i % S], (i / S) & 1, p.status, SB_DEVERR_DRAIN)) break;
       }
-      __syncwarp();
-    } else if (warp == 9) {
-      // ---------------------------------------------------------------- MMA
-      if (lane == 0) {
-        int it = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-          const F8Item w = f8_item(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t);
-          const bool second = kGate || w.n0 + C::kHalf < p.n;
-          const uint32_t idesc = idesc_e4m3_f32(C::kBM, second ? 2 * C::kHalf : C::kHalf);
-          for (int kk = 0; kk < nk; ++kk, ++it) {
-            const int s = it % S, buf = it & 1;
-            ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, p.status, SB_DEVERR_EPI_WAIT) &&
-                 mbar_wait(&full[s], (it / S) & 1, p.status, SB_DEVERR_TMA_WAIT);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t a_base = smem_u32(smem + C::kOffA + s * C::kABytes);
-            const uint32_t b_base = smem_u32(smem + C::kOffB + s * 2 * C::kHalfBytes);
+      // every stage released: all copies landed and all commit arrivals done
+      for (int i = it - S > 0 ? it - S : 0; i < it; ++i)
+        if (!mbar_wait(&empty[i % S], (i / S) & 1, p.status, SB_DEVERR_DRAIN)) break;
+    }
+    __syncwarp();
+    } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMA (a pair's leader)
+    if (lane == 0 && rank == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += stride) {
+        const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
+        const bool second = kGate || w.n0 + C::kHalf < p.n;
+        const uint32_t idesc = idesc_e4m3_f32(C::kItemRows, second ? 2 * C::kHalf : C::kHalf);
+        for (int kk = 0; kk < nk; ++kk, ++it) {
+          const int s = it % S, buf = it & 1;
+          ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, p.status, SB_DEVERR_EPI_WAIT) &&
+               mbar_wait(&full[s], (it / S) & 1, p.status, SB_DEVERR_TMA_WAIT);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(smem + C::kOffA + s * C::kABytes);
+          const uint32_t b_base = smem_u32(smem + C::kOffB + s * C::kBBytes);
 #pragma unroll
-            for (int q = 0; q < C::kBK / 32; ++q)
-              tc_mma_f8(tmem + buf * C::kAccCols, smem_desc_k_sw128(a_base + q * 32), smem_desc_k_sw128(b_base + q * 32),
-                        idesc, q > 0);
+          for (int q = 0; q < C::kBK / 32; ++q)
+            tc_mma_f8<kPair>(tmem + buf * C::kAccCols, smem_desc_k_sw128(a_base + q * 32),
+                             smem_desc_k_sw128(b_base + q * 32), idesc, q > 0);
+          if constexpr (kPair) {
+            tc_commit_pair(&empty[s]);
+            tc_commit_pair(&acc_full[buf]);
+          } else {
             tc_commit(&empty[s]);
             tc_commit(&acc_full[buf]);
           }
         }
       }
-      __syncwarp();
+    }
+    __syncwarp();
     }
   } else {
     // ---------------------------------------------------------------- epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsEpi));
+    constexpr int NC = C::kCols;
     const int quarter = warp & 3, part = warp >> 2;
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * 64;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * NC;
     uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
-    float* s_bs = reinterpret_cast<float*>(smem + C::kOffBScale) + warp * 128;
+    float* s_bs = reinterpret_cast<float*>(smem + C::kOffBScale) + warp * 2 * NC;
+    const uint32_t acc_empty_addr = kPair ? mapa_shared(smem_u32(acc_empty), 0) : 0;
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const F8Item w = f8_item(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t);
-      const int r = quarter * 32 + lane;          // row of the tile
+    for (int t = first; t < total && ok; t += stride) {
+      const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
+      const int r = quarter * 32 + lane;          // row of this CTA's tile
       const bool live = r < w.rows;
       const bool warp_live = quarter * 32 < w.rows;
+      const bool second = kGate || w.n0 + C::kHalf < p.n;
       const int64_t row = w.row0 + r;
       const float* sa_ptr = p.a_scale + row * p.a_scale_row;
       const float* sb0 = (kGate ? p.b_gate_scale : p.b_scale) + w.g * p.b_scale_group;
@@ -289,120 +405,189 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         sb0 += (w.n0 / 128) * p.b_scale_row;
         sb1 += (w.n0 / 128 + (kGate ? 0 : 1)) * p.b_scale_row;
       }
-      const bool second = kGate || w.n0 + C::kHalf < p.n;
-      // kBRows: lane i stages the scales of four of the warp's 128 columns
-      const int bcol = w.n0 + (lane >> 4) * C::kHalf + part * 64 + (lane & 15) * 4;
-      float acc[2][64];
+      // kBRows: a lane stages the scales of NC / 16 of the warp's 2 NC columns
+      constexpr int NB = NC / 16;
+      const int bcol = w.n0 + (lane >> 4) * C::kHalf + part * NC + (lane & 15) * NB;
+      uint64_t sum[2][NC / 2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 64; ++i) acc[h][i] = 0.f;
+        for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
+      // scales of block kk are loaded one block ahead: their latency is longer
+      // than a block's MMAs
+      float sa = live ? sa_ptr[0] : 0.f;
+      float p0 = 0.f, p1 = 0.f, pb[NB] = {};
+      auto load_b_scales = [&](int kk) {
+        if (kBRows) {
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+            if (bcol + j < p.n) pb[j] = sb1[(bcol + j) * p.b_scale_row + kk * p.b_scale_block];
+        } else {
+          p0 = sb0[kk * p.b_scale_block];
+          if (second) p1 = sb1[kk * p.b_scale_block];
+        }
+      };
+      load_b_scales(0);
       for (int kk = 0; kk < nk; ++kk, ++it) {
         const int buf = it & 1;
-        const float sa = live ? sa_ptr[kk * p.a_scale_block] : 0.f;
-        float s0 = 0.f, s1 = 0.f;
+        const uint64_t s0 = pair_of(kBRows ? sa : sa * p0), s1 = pair_of(kBRows ? sa : sa * p1);
         if (kBRows) {
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            s_bs[lane * 4 + j] = bcol + j < p.n ? sb1[(bcol + j) * p.b_scale_row + kk * p.b_scale_block] : 0.f;
+          for (int j = 0; j < NB; ++j) s_bs[lane * NB + j] = pb[j];
           __syncwarp();
-        } else {
-          s0 = sa * sb0[kk * p.b_scale_block];
-          if (second) s1 = sa * sb1[kk * p.b_scale_block];
+        }
+        if (kk + 1 < nk) {
+          if (live) sa = sa_ptr[(kk + 1) * p.a_scale_block];
+          load_b_scales(kk + 1);
         }
         if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const uint32_t t0 = lane_addr + buf * C::kAccCols;
+        constexpr int CH = C::kChunk;
+        constexpr int kLoads = 2 * NC / CH;
+        uint64_t v[CH / 2];
+        auto load = [&](int j) { tmem_ld_pairs<CH>(t0 + (j * CH / NC) * C::kHalf + j * CH % NC, v); };
+        auto add = [&](int j) {
+          const int h = j * CH / NC, c = j * CH % NC;
+#pragma unroll
+          for (int i = 0; i < CH / 2; ++i)
+            fma_pair(sum[h][c / 2 + i],
+                     kBRows ? mul_pair(v[i], *reinterpret_cast<const uint64_t*>(s_bs + h * NC + c + 2 * i)) : v[i],
+                     h ? s1 : s0);
+        };
         if (warp_live) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h == 1 && !second) break;
-            const float s = h ? s1 : s0;
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-              float v[32];
-              tmem_ld32(lane_addr + buf * C::kAccCols + h * C::kHalf + c, v);
-              if (kBRows) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[h][c + i] = fmaf(v[i] * s_bs[h * 64 + c + i], sa, acc[h][c + i]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[h][c + i] = fmaf(v[i], s, acc[h][c + i]);
-              }
+          for (int j = 0; j < kLoads - 1; ++j)
+            if (j * CH < NC || second) {
+              load(j);
+              add(j);
             }
-          }
+          if (second) load(kLoads - 1);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        if (lane == 0) {
+          if constexpr (kPair) mbar_arrive_leader(acc_empty_addr + 8u * buf);
+          else mbar_arrive(&acc_empty[buf]);
+        }
+        if (warp_live && second) add(kLoads - 1);
       }
+      float acc[2][NC];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i)
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[h][2 * i]), "=f"(acc[h][2 * i + 1]) : "l"(sum[h][i]));
       if constexpr (!kQuant) {
         if (!ok || !warp_live) continue;
         const float rs = live && p.row_scale ? p.row_scale[row] : 1.f;
+        // whole boxes of 32 rows leave through shared memory (the hardware clips
+        // columns past n); element stores would keep the warp, and with it the
+        // tensor core, waiting for 16-byte pieces of 32 different rows
+        const bool staged = kPair && tma_out && quarter * 32 + 32 <= w.rows;
+        uint8_t* box = smem + C::kOffOut + warp * 2 * C::kBoxBytes;
+        if (staged) {
+          if (lane == 0) tma_store_wait_read();  // the previous item's boxes have left
+          __syncwarp();
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int c0 = w.n0 + h * C::kHalf + part * 64;
+          const int c0 = w.n0 + h * C::kHalf + part * NC;
           const int valid = p.n - c0;
           if (valid <= 0) continue;
           if (p.bias) {
             const float* bias = p.bias + w.g * p.bias_group + c0;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[h][i] += i < valid ? bias[i] : 0.f;
+            for (int i = 0; i < NC; ++i) acc[h][i] += i < valid ? bias[i] : 0.f;
           }
 #pragma unroll
-          for (int i = 0; i < 64; ++i) acc[h][i] *= rs;
+          for (int i = 0; i < NC; ++i) acc[h][i] *= rs;
+          if (staged) {
+            if (p.out_dtype == SB_F32) {
+              if (h == 1) {
+                if (lane == 0) tma_store_wait_read();
+                __syncwarp();
+              }
+#pragma unroll
+              for (int i = 0; i < NC; i += 4)
+                *box_chunk(box + (i / 32) * C::kBoxBytes, lane, i % 32 / 4) =
+                    make_uint4(__float_as_uint(acc[h][i]), __float_as_uint(acc[h][i + 1]),
+                               __float_as_uint(acc[h][i + 2]), __float_as_uint(acc[h][i + 3]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < NC; i += 8)
+                *box_chunk(box + h * C::kBoxBytes, lane, i / 8) =
+                    make_uint4(bf16_pair(acc[h][i], acc[h][i + 1]), bf16_pair(acc[h][i + 2], acc[h][i + 3]),
+                               bf16_pair(acc[h][i + 4], acc[h][i + 5]), bf16_pair(acc[h][i + 6], acc[h][i + 7]));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              const int row0 = w.row0 + quarter * 32;
+              if (p.out_dtype == SB_F32) {
+                tma_store_2d(&tmO, box, c0, row0);
+                if (valid > 32) tma_store_2d(&tmO, box + C::kBoxBytes, c0 + 32, row0);
+              } else {
+                tma_store_2d(&tmO, box + h * C::kBoxBytes, c0, row0);
+              }
+            }
+            continue;
+          }
           if (!live) continue;
           if (p.out_dtype == SB_F32) {
             float* dst = static_cast<float*>(p.out) + row * p.ldo + c0;
-            store_row64(dst, acc[h], valid, reinterpret_cast<uintptr_t>(dst) % 16 == 0);
+            store_row(dst, acc[h], valid, reinterpret_cast<uintptr_t>(dst) % 16 == 0);
           } else {
             __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + c0;
-            store_row64(dst, acc[h], valid, reinterpret_cast<uintptr_t>(dst) % 16 == 0);
+            store_row(dst, acc[h], valid, reinterpret_cast<uintptr_t>(dst) % 16 == 0);
           }
         }
       } else {
-        // activation, then one 1 x 128 block per row (SwiGLU) or two (GELU),
-        // each held by this thread and the other part's thread of the same row
+        // activation, then one 1 x 128 block per row (SwiGLU) or two (GELU), each
+        // held by the threads of the row in the quarter's four warps
         constexpr int kBlocks = kGate ? 1 : 2;
-        uint32_t amax[kBlocks];
+        if (warp_live) {
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const int c0 = w.n0 + b * C::kHalf + part * 64;
-          const int valid = p.n - c0;
-          const float* bias = p.bias ? p.bias + w.g * p.bias_group + c0 : nullptr;
-          const float* bgate = kGate && p.bias_gate ? p.bias_gate + w.g * p.bias_group + c0 : nullptr;
-          uint32_t m = 0;
+          for (int b = 0; b < kBlocks; ++b) {
+            const int c0 = w.n0 + b * C::kHalf + part * NC;
+            const int valid = p.n - c0;
+            const float* bias = p.bias ? p.bias + w.g * p.bias_group + c0 : nullptr;
+            const float* bgate = kGate && p.bias_gate ? p.bias_gate + w.g * p.bias_group + c0 : nullptr;
+            uint32_t m = 0;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            float y;
-            if (kGate) {
-              const float up = acc[1][i] + (bias && i < valid ? bias[i] : 0.f);
-              y = silu(acc[0][i] + (bgate && i < valid ? bgate[i] : 0.f)) * up;
-            } else {
-              y = gelu_erf(acc[b][i] + (bias && i < valid ? bias[i] : 0.f));
+            for (int i = 0; i < NC; ++i) {
+              float y;
+              if (kGate) {
+                const float up = acc[1][i] + (bias && i < valid ? bias[i] : 0.f);
+                y = silu(acc[0][i] + (bgate && i < valid ? bgate[i] : 0.f)) * up;
+              } else {
+                y = gelu_erf(acc[b][i] + (bias && i < valid ? bias[i] : 0.f));
+              }
+              y = i < valid ? y : 0.f;
+              acc[b][i] = y;
+              m = max(m, abs_bits(y));
             }
-            y = i < valid ? y : 0.f;
-            acc[b][i] = y;
-            m = max(m, abs_bits(y));
+            s_max[(b * C::kParts + part) * C::kBM + r] = m;
           }
-          amax[b] = m;
-          s_max[(b * 2 + part) * C::kBM + r] = m;
         }
-        ok = named_bar_and(1 + quarter, 64, ok);
+        ok = named_bar_and(1 + quarter, 32 * C::kParts, ok);
         if (live && ok) {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
-            const int c0 = w.n0 + b * C::kHalf + part * 64;
+            const int c0 = w.n0 + b * C::kHalf + part * NC;
             if (w.n0 + b * C::kHalf >= p.n) continue;
-            const Fp8Scale s = fp8_scale(max(amax[b], s_max[(b * 2 + (part ^ 1)) * C::kBM + r]));
-            if (part == 0)
-              p.out_scale[row * p.out_scale_row + (w.n0 / 128 + b) * p.out_scale_block] = s.scale;
+            uint32_t m = 0;
+#pragma unroll
+            for (int q = 0; q < C::kParts; ++q) m = max(m, s_max[(b * C::kParts + q) * C::kBM + r]);
+            const Fp8Scale s = fp8_scale(m);
+            if (part == 0) p.out_scale[row * p.out_scale_row + (w.n0 / 128 + b) * p.out_scale_block] = s.scale;
             uint8_t* dst = static_cast<uint8_t*>(p.out) + row * p.ldo + c0;
 #pragma unroll
-            for (int i = 0; i < 64; i += 16) {
+            for (int i = 0; i < NC; i += 16) {
               uint32_t q[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
@@ -418,33 +603,61 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             }
           }
         }
-        named_bar_sync(1 + quarter, 64);  // s_max is free for the next item
+        named_bar_sync(1 + quarter, 32 * C::kParts);  // s_max is free for the next item
       }
     }
   }
+  if (kPair && !kQuant && warp < C::kEpiWarps && lane == 0) tma_store_wait_all();  // stores done before the CTA leaves
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
-  if (warp == 9) {
+  if constexpr (kPair) cluster_sync();  // neither CTA leaves while the other may still signal it
+  else __syncthreads();
+  if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::kTmemCols);
+    if constexpr (kPair) tmem_dealloc_pair(tmem, C::kTmemCols);
+    else tmem_dealloc(tmem, C::kTmemCols);
   }
 }
 
 static bool f8_map(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int64_t pitch, int box_rows) {
-  return make_map(m, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, k, rows, pitch, F8Cfg::kBK, box_rows,
-                  CU_TENSOR_MAP_SWIZZLE_128B);
+  return make_map(m, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, k, rows, pitch, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int EPI, bool kBRows>
+template <int EPI, bool kBRows, bool kPair>
 static int launch_f8(const sb_fp8_matmul_args& a, cudaStream_t st) {
-  using C = F8Cfg;
-  auto kern = f8_gemm_kernel<EPI, kBRows>;
+  using C = F8Cfg<kPair>;
+  auto kern = f8_gemm_kernel<EPI, kBRows, kPair>;
   static int configured_device = -1;
+  static int max_ctas = 0;  // CTAs (or pairs) that run at once
   int dev = 0;
   cudaGetDevice(&dev);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
   if (configured_device != dev) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess) return cuda_status(e);
+    int n = current_sm_count();
+    if (kPair) {
+      cfg.gridDim = dim3(2 * n);
+      cfg.attrs = attr + 1;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters <= 0) {
+        cudaGetLastError();
+        clusters = n / 2;
+      }
+      n = clusters;
+    }
+    max_ctas = n;
     configured_device = dev;
   }
   constexpr int kTileCols = EPI == SB_EPI_SWIGLU ? C::kHalf : 2 * C::kHalf;
@@ -455,13 +668,27 @@ static int launch_f8(const sb_fp8_matmul_args& a, cudaStream_t st) {
     return SB_ERR_UNSUPPORTED;
   mg = mb;
   if (EPI == SB_EPI_SWIGLU && !f8_map(&mg, a.b_gate, a.k, b_rows, a.ldb, C::kHalf)) return SB_ERR_UNSUPPORTED;
+  // LINEAR outputs of the pair schedule as a tensor of boxes of 32 rows x 128
+  // bytes; without one (an unaligned output) every element is stored by its thread
+  CUtensorMap mo = ma;
+  const int esize = a.out_dtype == SB_F32 ? 4 : 2;
+  const int tma_out =
+      kPair && EPI == SB_EPI_LINEAR && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * esize % 16 == 0 &&
+      make_map(&mo, a.out, esize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n,
+               a.max_rows, a.ldo * esize, 128 / esize, 32, CU_TENSOR_MAP_SWIZZLE_128B);
   const int64_t n_tiles = (a.n + kTileCols - 1) / kTileCols;
-  const int64_t row_tiles = (a.max_rows + C::kBM - 1) / C::kBM + (a.offsets ? a.num_groups : 0);
+  const int64_t row_tiles = (a.max_rows + C::kItemRows - 1) / C::kItemRows + (a.offsets ? a.num_groups : 0);
   if (n_tiles * row_tiles > 0x7fffffff) return SB_ERR_UNSUPPORTED;
-  const int64_t sms = current_sm_count();
-  const int grid = static_cast<int>(n_tiles * row_tiles < sms ? n_tiles * row_tiles : sms);
-  return launch(kern, dim3(grid), dim3(C::kThreads), C::kSmemBytes, st, ma, mas, mb, mg, a);
+  const int ctas = static_cast<int>(n_tiles * row_tiles < max_ctas ? n_tiles * row_tiles : max_ctas);
+  cfg.gridDim = dim3(kPair ? 2 * ctas : ctas);
+  cfg.attrs = pdl_enabled() ? attr : attr + 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (kPair ? 1 : 0);
+  note_launch();
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, ma, mas, mb, mg, mo, a, tma_out));
 }
+
+// Pairs pay when the rows per group fill their 256-row tiles.
+static bool use_pair(const sb_fp8_matmul_args& a) { return a.max_rows / a.num_groups > 128; }
 
 }  // namespace sb
 
@@ -472,7 +699,7 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
   const sb_fp8_matmul_args& a = *args;
   const bool quant = a.epilogue == SB_EPI_GELU || a.epilogue == SB_EPI_SWIGLU;
   if ((!quant && a.epilogue != SB_EPI_LINEAR) || (!quant && a.out_dtype != SB_F32 && a.out_dtype != SB_BF16) ||
-      a.num_groups < 1 || a.num_groups > F8Cfg::kMaxG || (!a.offsets && a.num_groups != 1) || a.max_rows < 0 ||
+      a.num_groups < 1 || a.num_groups > kF8MaxG || (!a.offsets && a.num_groups != 1) || a.max_rows < 0 ||
       a.n < 1 || a.k < 1 || (a.b_block_rows != 128 && a.b_block_rows != 1) || (quant && a.b_block_rows != 128) ||
       a.lda < a.k || a.lda % 16 || a.ldb < a.k || a.ldb % 16 || (a.num_groups > 1 && a.b_group_rows < a.n) ||
       a.ldo < a.n || (quant && a.ldo % 16))
@@ -485,9 +712,13 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
   if ((a.num_groups - 1) * a.b_group_rows + a.n > 0x7fffffff) return SB_ERR_UNSUPPORTED;  // TMA row coordinates
   if (current_cc_major() != 10) return SB_ERR_NO_DEVICE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.epilogue == SB_EPI_SWIGLU) return launch_f8<SB_EPI_SWIGLU, false>(a, st);
-  if (a.epilogue == SB_EPI_GELU) return launch_f8<SB_EPI_GELU, false>(a, st);
-  return a.b_block_rows == 1 ? launch_f8<SB_EPI_LINEAR, true>(a, st) : launch_f8<SB_EPI_LINEAR, false>(a, st);
+  const bool pair = use_pair(a);
+#define SB_F8(EPI, ROWS) return pair ? launch_f8<EPI, ROWS, true>(a, st) : launch_f8<EPI, ROWS, false>(a, st)
+  if (a.epilogue == SB_EPI_SWIGLU) SB_F8(SB_EPI_SWIGLU, false);
+  if (a.epilogue == SB_EPI_GELU) SB_F8(SB_EPI_GELU, false);
+  if (a.b_block_rows == 1) SB_F8(SB_EPI_LINEAR, true);
+  SB_F8(SB_EPI_LINEAR, false);
+#undef SB_F8
 }
 
 // ------------------------------------------------------------------ expert delta
@@ -504,7 +735,7 @@ struct F8DeltaBuffers {
 };
 
 static bool f8_experts_ok(const sb_fp8_experts* x) {
-  return x && x->num_experts >= 1 && x->num_experts <= F8Cfg::kMaxG && x->hidden >= 1 && x->ffn >= 1 &&
+  return x && x->num_experts >= 1 && x->num_experts <= kF8MaxG && x->hidden >= 1 && x->ffn >= 1 &&
          (x->activation == SB_ACT_GELU || x->activation == SB_ACT_SWIGLU) && x->ld_in % 16 == 0 && x->ld_in >= x->hidden &&
          x->ld_ffn % 16 == 0 && x->ld_ffn >= x->ffn;
 }
