@@ -563,9 +563,9 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               float y;
               if (kGate) {
                 const float up = acc[1][i] + (bias && i < valid ? bias[i] : 0.f);
-                y = silu(acc[0][i] + (bgate && i < valid ? bgate[i] : 0.f)) * up;
+                y = silu_bf16out(acc[0][i] + (bgate && i < valid ? bgate[i] : 0.f)) * up;
               } else {
-                y = gelu_erf(acc[b][i] + (bias && i < valid ? bias[i] : 0.f));
+                y = gelu_bf16out(acc[b][i] + (bias && i < valid ? bias[i] : 0.f));
               }
               y = i < valid ? y : 0.f;
               acc[b][i] = y;
@@ -616,6 +616,386 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     tc_fence_after();
     if constexpr (kPair) tmem_dealloc_pair(tmem, C::kTmemCols);
     else tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+//
+// Decode batches: a handful of rows per group, weights streamed once.  The roles
+// are swapped: 128 weight rows are the MMA's M side (the TMEM lanes), the kN
+// token rows its N side, so scaling and adding a block's kN columns is spread
+// over all four lane quarters instead of over the one quarter that a few token
+// rows fill (measured on 128 experts x 2048 x 768 at 16 rows each: the up product
+// 137 us with rows as M).  A thread holds one output feature and half of the
+// token columns; a SwiGLU item has a gate and an up tile, so the thread has both.
+// Row tiles of a group are neighbours in the schedule, so their weight tiles
+// meet in L2.
+//
+// LINEAR problems with fewer items than SMs split k over the CTAs of a cluster,
+// whose partial sums are added in rank order through distributed shared memory:
+// one launch, no workspace, the same result every time.
+//
+// Warps: 0-7 epilogue (quarter w % 4, columns half w / 4), 8 TMA, 9 MMA (+TMEM).
+template <int EPI, int kN>
+struct F8DecCfg {
+  static constexpr bool kGate = EPI == SB_EPI_SWIGLU;
+  static constexpr int kTiles = kGate ? 2 : 1;  // 128-row weight tiles per item
+  static constexpr int kWBytes = 128 * 128;
+  static constexpr int kXBytes = kN * 128;
+  static constexpr int kStageBytes = kTiles * kWBytes + kXBytes;
+  static constexpr int kStagesRaw = (190 * 1024) / kStageBytes;
+  static constexpr int kStages = kStagesRaw > 10 ? 10 : kStagesRaw;
+  static constexpr int kAcc = 4;  // accumulators in flight between the MMAs and the epilogue
+  static constexpr int kAccCols = kTiles * kN;
+  static constexpr int kTmemCols = kAcc * kAccCols < 32 ? 32 : kAcc * kAccCols;
+  static constexpr int kThreads = 320;
+  static constexpr int kCols = kN / 2;  // columns per epilogue thread and tile
+  static constexpr int kOffX = kStages * kTiles * kWBytes;
+  static constexpr int kOffBar = kOffX + kStages * kXBytes;
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + 2 * kAcc) * 8;
+  static constexpr int kOffFactor = (kOffMisc + 16 + 15) / 16 * 16;        // float [8 warps][kTiles][kCols]
+  static constexpr int kOffMax = kOffFactor + 8 * kTiles * kCols * 4;      // uint32 [kN][4 quarters]
+  static constexpr int kOffPrefix = kOffMax + kN * 4 * 4;
+  static constexpr int kOffOffsets = kOffPrefix + (kF8MaxG + 1) * 4;
+  static constexpr int kSmemBytes = kOffOffsets + (kF8MaxG + 1) * 4 + 1024;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+  static_assert(kTmemCols <= 512, "accumulators");
+  static_assert(kTiles * kN * 128 * 4 <= kOffX, "the split's partial sums reuse the weight stages");
+};
+
+template <int kN>
+SB_DEVINL void tmem_ld_cols(uint32_t taddr, uint64_t (&v)[kN / 2]) {
+  if constexpr (kN == 8) {
+    uint32_t r[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("mov.b64 %0, {%1, %2};" : "=l"(v[i]) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+  } else {
+    tmem_ld_pairs<kN>(taddr, v);
+  }
+}
+SB_DEVINL float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Item t -> group, first row, valid rows, first feature; row tiles fastest.
+template <int kN>
+SB_DEVINL F8Item f8_dec_item(const int* prefix, const int* s_off, int G, int n_tiles, int max_rows, int t) {
+  int lo = 0, hi = G - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  const int local = t - prefix[lo];
+  const int end = min(s_off[lo + 1], max_rows);
+  const int row_tiles = (end - s_off[lo] + kN - 1) / kN;
+  const int nt = local / row_tiles;
+  F8Item i;
+  i.g = lo;
+  i.row0 = s_off[lo] + (local - nt * row_tiles) * kN;
+  i.rows = min(end - i.row0, kN);
+  i.peer = 0;
+  i.n0 = nt * 128;
+  return i;
+}
+
+template <int EPI, int kN>
+__global__ void __launch_bounds__(F8DecCfg<EPI, kN>::kThreads, 1)
+f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                 const __grid_constant__ CUtensorMap tmG, const sb_fp8_matmul_args p, const int splits) {
+  using C = F8DecCfg<EPI, kN>;
+  constexpr int S = C::kStages, NT = C::kTiles, NC = C::kCols;
+  constexpr bool kGate = C::kGate;
+  constexpr bool kQuant = EPI != SB_EPI_LINEAR;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;
+  uint64_t* acc_empty = acc_full + C::kAcc;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
+  int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = static_cast<int>(blockIdx.x) % splits;  // splits == cluster size
+  const int first = static_cast<int>(blockIdx.x) / splits, stride = static_cast<int>(gridDim.x) / splits;
+  const int G = p.num_groups;
+  const int n_tiles = (p.n + 127) / 128;
+  const int nk_all = (p.k + 127) / 128;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(nk_all) * rank / splits);
+  const int nk = static_cast<int>(static_cast<int64_t>(nk_all) * (rank + 1) / splits) - kb0;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < C::kAcc; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+    if (kGate) tma_prefetch_desc(&tmG);
+  }
+  if (warp == 9) {
+    tmem_alloc(s_tmem, C::kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {
+    int seen = 0;
+    for (int base = 0; base < G; base += 32) {
+      const int gi = base + lane;
+      int tiles = 0;
+      if (gi < G) {
+        const int o0 = group_offset(p.offsets, gi, p.max_rows), o1 = group_offset(p.offsets, gi + 1, p.max_rows);
+        s_off[gi] = o0;
+        if (gi == G - 1) s_off[G] = o1;
+        const int lo = min(o0, p.max_rows), hi = min(o1, p.max_rows);
+        tiles = hi > lo ? (hi - lo + kN - 1) / kN * n_tiles : 0;
+      }
+      int incl = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += t;
+      }
+      if (gi < G) prefix[gi] = seen + incl - tiles;
+      seen += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) prefix[G] = seen;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const int total = prefix[G];
+  bool ok = true;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0) {
+      int it = 0;
+      for (int t = first; t < total && ok; t += stride) {
+        const F8Item w = f8_dec_item<kN>(prefix, s_off, G, n_tiles, p.max_rows, t);
+        const int wrow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
+        for (int kk = 0; kk < nk; ++kk, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
+          mbar_expect_tx(&full[s], C::kStageBytes);
+          const int k0 = (kb0 + kk) * 128;
+          uint8_t* wdst = smem + s * NT * C::kWBytes;
+          if (kGate) tma_load_2d(wdst, &tmG, &full[s], k0, wrow);
+          tma_load_2d(wdst + (NT - 1) * C::kWBytes, &tmW, &full[s], k0, wrow);
+          tma_load_2d(smem + C::kOffX + s * C::kXBytes, &tmX, &full[s], k0, w.row0);
+        }
+      }
+      for (int i = it - S > 0 ? it - S : 0; i < it; ++i)
+        if (!mbar_wait(&empty[i % S], (i / S) & 1, p.status, SB_DEVERR_DRAIN)) break;
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(128, kN);
+      int it = 0;
+      for (int t = first; t < total && ok; t += stride) {
+        for (int kk = 0; kk < nk; ++kk, ++it) {
+          const int s = it % S, buf = it % C::kAcc;
+          ok = mbar_wait(&acc_empty[buf], ((it / C::kAcc) & 1) ^ 1, p.status, SB_DEVERR_EPI_WAIT) &&
+               mbar_wait(&full[s], (it / S) & 1, p.status, SB_DEVERR_TMA_WAIT);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t w_base = smem_u32(smem + s * NT * C::kWBytes);
+          const uint32_t x_base = smem_u32(smem + C::kOffX + s * C::kXBytes);
+#pragma unroll
+          for (int h = 0; h < NT; ++h)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              tc_mma_f8<false>(tmem + buf * C::kAccCols + h * kN, smem_desc_k_sw128(w_base + h * C::kWBytes + q * 32),
+                               smem_desc_k_sw128(x_base + q * 32), idesc, q > 0);
+          tc_commit(&empty[s]);
+          tc_commit(&acc_full[buf]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * NC;
+    float* s_f = reinterpret_cast<float*>(smem + C::kOffFactor) + warp * NT * NC;
+    uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
+    float* s_red = reinterpret_cast<float*>(smem);  // [kN][128], splits > 1 only
+    int it = 0;
+    for (int t = first; t < total && ok; t += stride) {
+      const F8Item w = f8_dec_item<kN>(prefix, s_off, G, n_tiles, p.max_rows, t);
+      const int feat = w.n0 + quarter * 32 + lane;
+      const bool fvalid = feat < p.n;
+      const bool warp_live = half * NC < w.rows;  // some token column of this warp is valid
+      // lane i (mod NC) stages the factors of column i of each tile
+      const int scol = half * NC + lane % NC;
+      const bool sc_live = lane < NC && scol < w.rows;
+      const float* sa_ptr = p.a_scale + static_cast<int64_t>(w.row0 + (sc_live ? scol : 0)) * p.a_scale_row +
+                            kb0 * p.a_scale_block;
+      const int64_t wofs = w.g * p.b_scale_group + (w.n0 / 128) * p.b_scale_row + kb0 * p.b_scale_block;
+      const float* sw_ptr = p.b_scale + wofs;
+      const float* sg_ptr = kGate ? p.b_gate_scale + wofs : nullptr;
+      uint64_t sum[NT][NC / 2];
+#pragma unroll
+      for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
+      float sa = 0.f, sw = 0.f, sg = 0.f;
+      auto load_scales = [&](int kk) {
+        if (sc_live) sa = sa_ptr[kk * p.a_scale_block];
+        sw = sw_ptr[kk * p.b_scale_block];
+        if (kGate) sg = sg_ptr[kk * p.b_scale_block];
+      };
+      if (nk > 0) load_scales(0);
+      for (int kk = 0; kk < nk; ++kk, ++it) {
+        const int buf = it % C::kAcc;
+        __syncwarp();
+        if (lane < NC) {
+          if (kGate) s_f[lane] = sa * sg;
+          s_f[(NT - 1) * NC + lane] = sa * sw;
+        }
+        __syncwarp();
+        if (kk + 1 < nk) load_scales(kk + 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it / C::kAcc) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_live) {
+#pragma unroll
+          for (int h = 0; h < NT; ++h) {
+            uint64_t v[NC / 2];
+            tmem_ld_cols<NC>(lane_addr + buf * C::kAccCols + h * kN, v);
+            if (h == NT - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            }
+#pragma unroll
+            for (int i = 0; i < NC / 2; i += 2) {
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + h * NC + 2 * i);
+              fma_pair(sum[h][i], v[i], f.x);
+              fma_pair(sum[h][i + 1], v[i + 1], f.y);
+            }
+          }
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+      }
+      float acc[NT][NC];
+#pragma unroll
+      for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i)
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[h][2 * i]), "=f"(acc[h][2 * i + 1]) : "l"(sum[h][i]));
+      const float bias = p.bias && fvalid ? p.bias[w.g * p.bias_group + feat] : 0.f;
+      auto store_linear = [&](int col, float v) {
+        const int64_t row = w.row0 + col;
+        v += bias;
+        if (p.row_scale) v *= p.row_scale[row];
+        if (!fvalid) return;
+        if (p.out_dtype == SB_F32) static_cast<float*>(p.out)[row * p.ldo + feat] = v;
+        else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + feat] = __float2bfloat16_rn(v);
+      };
+      if constexpr (!kQuant) {
+        if (splits > 1) {
+          // this CTA's partial sums; every CTA of the cluster then finishes kN /
+          // splits columns.  One item per cluster, so the ring is done with.
+#pragma unroll
+          for (int i = 0; i < NC; ++i) s_red[(half * NC + i) * 128 + quarter * 32 + lane] = acc[0][i];
+          break;  // finished below, after the cluster's barrier
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          if (half * NC + i >= w.rows) break;
+          store_linear(half * NC + i, acc[0][i]);
+        }
+      } else {
+        const float bgate = kGate && p.bias_gate && fvalid ? p.bias_gate[w.g * p.bias_group + feat] : 0.f;
+        float y[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const float x = acc[NT - 1][i] + bias;
+          y[i] = kGate ? silu_bf16out(acc[0][i] + bgate) * x : gelu_bf16out(x);
+          if (!fvalid) y[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          if (half * NC + i >= w.rows) break;
+          const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(y[i]));
+          if (lane == 0) s_max[(half * NC + i) * 4 + quarter] = m;
+        }
+        ok = named_bar_and(1 + half, 128, ok);
+        if (ok) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            const int col = half * NC + i;
+            if (col >= w.rows) break;
+            const uint4 m = *reinterpret_cast<const uint4*>(s_max + col * 4);
+            const Fp8Scale sc = fp8_scale(max(max(m.x, m.y), max(m.z, m.w)));
+            const int64_t row = w.row0 + col;
+            if (quarter == 0 && lane == 0) p.out_scale[row * p.out_scale_row + (w.n0 / 128) * p.out_scale_block] = sc.scale;
+            if (fvalid)
+              static_cast<uint8_t*>(p.out)[row * p.ldo + feat] =
+                  static_cast<uint8_t>(fp8_pack4(y[i] * sc.inv, 0.f, 0.f, 0.f));
+          }
+        }
+        named_bar_sync(1 + half, 128);  // s_max is free for the next item
+      }
+    }
+  }
+  __syncwarp();
+  if (!kQuant && splits > 1) {
+    // every CTA of the cluster has its partial sums in place (each has an item:
+    // the grid is items x splits for plain products, whose item count the host knows)
+    cluster_sync();
+    if (warp < 8 && first < total) {
+      const F8Item w = f8_dec_item<kN>(prefix, s_off, G, n_tiles, p.max_rows, first);
+      const int quarter = warp & 3, half = warp >> 2;
+      const int feat = w.n0 + quarter * 32 + lane;
+      const float bias = p.bias && feat < p.n ? p.bias[w.g * p.bias_group + feat] : 0.f;
+      // columns rank, rank + splits, ...: alternately for the two halves' warps
+      for (int col = rank + half * splits; col < w.rows; col += 2 * splits) {
+        const uint32_t mine = smem_u32(smem) + (col * 128 + quarter * 32 + lane) * 4;
+        float v = 0.f;
+        for (int q = 0; q < splits; ++q) v += ld_cluster_f32(mapa_shared(mine, q));
+        const int64_t row = w.row0 + col;
+        v += bias;
+        if (p.row_scale) v *= p.row_scale[row];
+        if (feat < p.n) {
+          if (p.out_dtype == SB_F32) static_cast<float*>(p.out)[row * p.ldo + feat] = v;
+          else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + feat] = __float2bfloat16_rn(v);
+        }
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
   }
 }
 
@@ -687,6 +1067,61 @@ static int launch_f8(const sb_fp8_matmul_args& a, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, ma, mas, mb, mg, mo, a, tma_out));
 }
 
+template <int EPI, int kN>
+static int launch_f8_decode(const sb_fp8_matmul_args& a, cudaStream_t st) {
+  using C = F8DecCfg<EPI, kN>;
+  auto kern = f8_decode_kernel<EPI, kN>;
+  static int configured_device = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_device != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    if (e != cudaSuccess) return cuda_status(e);
+    configured_device = dev;
+  }
+  const int64_t b_rows = (a.num_groups - 1) * a.b_group_rows + a.n;
+  CUtensorMap mx, mw, mg;
+  if (!f8_map(&mx, a.a, a.k, a.max_rows, a.lda, kN) || !f8_map(&mw, a.b, a.k, b_rows, a.ldb, 128))
+    return SB_ERR_UNSUPPORTED;
+  mg = mw;
+  if (EPI == SB_EPI_SWIGLU && !f8_map(&mg, a.b_gate, a.k, b_rows, a.ldb, 128)) return SB_ERR_UNSUPPORTED;
+  const int64_t n_tiles = (a.n + 127) / 128;
+  const int64_t row_tiles = (a.max_rows + kN - 1) / kN + (a.offsets ? (a.num_groups < a.max_rows ? a.num_groups : a.max_rows) : 0);
+  const int64_t items = n_tiles * row_tiles;
+  if (items > 0x7fffffff) return SB_ERR_UNSUPPORTED;
+  const int sms = current_sm_count();
+  // k split over clusters of 2, 4 or 8 CTAs while they all fit the GPU at once,
+  // with at least two blocks of k each
+  int splits = 1;
+  if (EPI == SB_EPI_LINEAR && !a.offsets)
+    while (splits < 8 && items * splits * 2 <= sms && (a.k + 127) / 128 >= 4 * splits) splits *= 2;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits > 1 ? static_cast<int>(items) * splits : static_cast<int>(items < sms ? items : sms));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cfg.attrs = pdl_enabled() ? attr : attr + 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (splits > 1 ? 1 : 0);
+  note_launch();
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, mx, mw, mg, a, splits));
+}
+
+// Rows per group (of a plain product: rows) up to which the weights-as-M
+// schedule runs, and its column count.
+static int decode_columns(const sb_fp8_matmul_args& a) {
+  if (a.b_block_rows != 128) return 0;
+  if (!a.offsets) return a.max_rows <= 16 ? 16 : (a.max_rows <= 32 ? 32 : (a.max_rows <= 64 ? 64 : 0));
+  const int per_group = a.max_rows / a.num_groups;
+  return per_group <= 4 ? 16 : (per_group <= 20 ? 32 : (per_group <= 48 ? 64 : 0));
+}
+
 // Pairs pay when the rows per group fill their 256-row tiles.
 static bool use_pair(const sb_fp8_matmul_args& a) { return a.max_rows / a.num_groups > 128; }
 
@@ -712,6 +1147,18 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
   if ((a.num_groups - 1) * a.b_group_rows + a.n > 0x7fffffff) return SB_ERR_UNSUPPORTED;  // TMA row coordinates
   if (current_cc_major() != 10) return SB_ERR_NO_DEVICE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define SB_F8_DECODE(EPI)                                         \
+  do {                                                            \
+    if (cols == 16) return launch_f8_decode<EPI, 16>(a, st);      \
+    if (cols == 32) return launch_f8_decode<EPI, 32>(a, st);      \
+    return launch_f8_decode<EPI, 64>(a, st);                      \
+  } while (0)
+  if (const int cols = decode_columns(a)) {
+    if (a.epilogue == SB_EPI_SWIGLU) SB_F8_DECODE(SB_EPI_SWIGLU);
+    if (a.epilogue == SB_EPI_GELU) SB_F8_DECODE(SB_EPI_GELU);
+    SB_F8_DECODE(SB_EPI_LINEAR);
+  }
+#undef SB_F8_DECODE
   const bool pair = use_pair(a);
 #define SB_F8(EPI, ROWS) return pair ? launch_f8<EPI, ROWS, true>(a, st) : launch_f8<EPI, ROWS, false>(a, st)
   if (a.epilogue == SB_EPI_SWIGLU) SB_F8(SB_EPI_SWIGLU, false);
