@@ -292,6 +292,23 @@ typedef struct sb_fp8_matmul_args {
 
 SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream);
 
+/* Linear layer y = x w^T on that product: x [m, k] (dtype, row pitch ldx) is
+ * quantised here; w is a matrix [n, k] of w_dtype SB_F32 / SB_BF16 with row pitch
+ * ldw (quantised here too, w_scale NULL) or, with w_scale given, e4m3 with byte
+ * pitch ldw and 128 x 128 block scales of strides w_scale_row / w_scale_col.
+ * y [m, n] contiguous, in x's dtype.
+ * The backward pass: dx = dy w [m, k] (may be NULL to skip) and dw = dy^T x [n, k]
+ * (may be NULL), contiguous, in x's and w's dtype; dy in x's dtype with any
+ * strides; every operand quantised along the dimension its product sums over. */
+SB_API size_t sb_fp8_linear_workspace_bytes(int m, int n, int k, int packed);
+SB_API int sb_fp8_linear(const void* x, int dtype, int64_t ldx, int m, int n, int k, const void* w, int w_dtype,
+                         int64_t ldw, const float* w_scale, int64_t w_scale_row, int64_t w_scale_col, void* y,
+                         int* status, void* workspace, size_t workspace_bytes, void* stream);
+SB_API size_t sb_fp8_linear_backward_workspace_bytes(int m, int n, int k);
+SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t ldx, int m, int n, int k, const void* w,
+                                  int w_dtype, int64_t ldw, const void* dy, int64_t dy_row, int64_t dy_col, void* dx,
+                                  void* dw, int* status, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The routed experts' FFNs with block-scaled weights: sb_expert_delta for this
  * format.  Weights [E, ffn, hidden] (up, gate) and [E, hidden, ffn] (down) in
  * e4m3 with byte pitches ld_in / ld_ffn per row (multiples of 16), scales

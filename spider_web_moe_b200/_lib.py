@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes as C
 import os
 
+import torch
+
 from . import build as _build
 
 SB_OK = 0
@@ -126,6 +128,11 @@ SIGNATURES = {
     "sb_route_experts_backward": (i32, [vp, i32, i64, i32, i32, i32, i32, vp, i32, f32, vp, vp, vp, i64, vp]),
     "sb_fp8_quantize_blocks": (i32, [C.POINTER(Fp8QuantizeArgs), vp]),
     "sb_fp8_matmul": (i32, [C.POINTER(Fp8MatmulArgs), vp]),
+    "sb_fp8_linear_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "sb_fp8_linear": (i32, [vp, i32, i64, i32, i32, i32, vp, i32, i64, vp, i64, i64, vp, vp, vp, sz, vp]),
+    "sb_fp8_linear_backward_workspace_bytes": (sz, [i32, i32, i32]),
+    "sb_fp8_linear_backward": (i32, [vp, i32, i64, i32, i32, i32, vp, i32, i64, vp, i64, i64, vp, vp, vp, vp, sz,
+                                     vp]),
     "sb_fp8_expert_delta_workspace_bytes": (sz, [C.POINTER(Fp8Experts), i32, i32]),
     "sb_fp8_expert_delta": (i32, [C.POINTER(Fp8Experts), vp, i32, i64, vp, vp, i32, i32, vp, i32, vp, vp, sz, vp]),
     "sb_group_workspace_bytes": (sz, [i32, i32, i32]),
@@ -229,3 +236,14 @@ def ptr(t) -> int | None:
     if t is None:
         return None
     return t.data_ptr()
+
+
+def on_device(device, call):
+    """call(raw stream pointer of the device's current stream), with that device
+    current (the library launches on the current device)."""
+    index = device.index
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
+        return call(stream)
+    with torch.cuda.device(index):
+        return call(stream)

@@ -1168,6 +1168,127 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
 #undef SB_F8
 }
 
+// ------------------------------------------------------------------ linear layer
+namespace sb {
+
+// A quantised matrix in the workspace: rows x cols with 1 x 128 or 128 x 128 blocks.
+struct F8Buf {
+  uint8_t* q;
+  float* s;
+  int64_t ld, s_row, s_col;
+};
+static F8Buf f8_buf(Carver& c, int rows, int cols, int block_rows) {
+  F8Buf b;
+  const int64_t cb = (cols + 127) / 128;
+  b.ld = align_up(cols, 16);
+  b.q = c.take<uint8_t>(static_cast<size_t>(rows) * b.ld);
+  if (block_rows == 1) {
+    b.s_row = 1;
+    b.s_col = align_up(rows, 4);
+    b.s = c.take<float>(b.s_col * cb);
+  } else {
+    b.s_row = cb;
+    b.s_col = 1;
+    b.s = c.take<float>(static_cast<size_t>((rows + 127) / 128) * cb);
+  }
+  return b;
+}
+static int f8_quantize(const F8Buf& b, const void* x, int dtype, int rows, int cols, int64_t x_row, int64_t x_col,
+                       int block_rows, void* stream) {
+  sb_fp8_quantize_args q = {};
+  q.x = x; q.dtype = dtype; q.block_rows = block_rows; q.batch = 1; q.rows = rows; q.cols = cols;
+  q.x_row = x_row; q.x_col = x_col; q.q = b.q; q.ldq = b.ld;
+  q.scale = b.s; q.scale_row = b.s_row; q.scale_col = b.s_col;
+  return sb_fp8_quantize_blocks(&q, stream);
+}
+static int f8_product(const F8Buf& a, const F8Buf& b, int b_block_rows, int m, int n, int k, void* out, int out_dtype,
+                      int* status, void* stream) {
+  sb_fp8_matmul_args g = {};
+  g.epilogue = SB_EPI_LINEAR; g.out_dtype = out_dtype; g.num_groups = 1; g.max_rows = m; g.n = n; g.k = k;
+  g.a = a.q; g.lda = a.ld; g.a_scale = a.s; g.a_scale_row = a.s_row; g.a_scale_block = a.s_col;
+  g.b = b.q; g.ldb = b.ld; g.b_scale = b.s; g.b_scale_row = b.s_row; g.b_scale_block = b.s_col;
+  g.b_block_rows = b_block_rows; g.out = out; g.ldo = n; g.status = status;
+  return sb_fp8_matmul(&g, stream);
+}
+static bool f8_linear_ok(int dtype, int64_t ldx, int m, int n, int k, int w_dtype) {
+  return (dtype == SB_F32 || dtype == SB_BF16) && (w_dtype == SB_F32 || w_dtype == SB_BF16) && m >= 0 && n >= 1 &&
+         k >= 1 && ldx >= k;
+}
+
+}  // namespace sb
+
+extern "C" SB_API size_t sb_fp8_linear_workspace_bytes(int m, int n, int k, int packed) {
+  if (m < 0 || n < 1 || k < 1) return 0;
+  Carver c(nullptr, ~size_t(0) >> 1);
+  f8_buf(c, m, k, 1);
+  if (!packed) f8_buf(c, n, k, 128);
+  return align_up(c.used, 256) + 256;
+}
+
+extern "C" SB_API int sb_fp8_linear(const void* x, int dtype, int64_t ldx, int m, int n, int k, const void* w,
+                                    int w_dtype, int64_t ldw, const float* w_scale, int64_t w_scale_row,
+                                    int64_t w_scale_col, void* y, int* status, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (!f8_linear_ok(dtype, ldx, m, n, k, w_dtype) || ldw < k || !w) return SB_ERR_ARG;
+  if (m == 0) return SB_OK;
+  if (!x || !y) return SB_ERR_ARG;
+  Carver c(workspace, workspace_bytes);
+  const F8Buf xq = f8_buf(c, m, k, 1);
+  F8Buf wq;
+  if (w_scale) {
+    wq = {const_cast<uint8_t*>(static_cast<const uint8_t*>(w)), const_cast<float*>(w_scale), ldw, w_scale_row,
+          w_scale_col};
+  } else {
+    wq = f8_buf(c, n, k, 128);
+  }
+  if (!workspace || c.overflow) return SB_ERR_WORKSPACE;
+  if (!w_scale) {
+    const int rc = f8_quantize(wq, w, w_dtype, n, k, ldw, 1, 128, stream);
+    if (rc) return rc;
+  }
+  const int rc = f8_quantize(xq, x, dtype, m, k, ldx, 1, 1, stream);
+  return rc ? rc : f8_product(xq, wq, 128, m, n, k, y, dtype, status, stream);
+}
+
+extern "C" SB_API size_t sb_fp8_linear_backward_workspace_bytes(int m, int n, int k) {
+  if (m < 0 || n < 1 || k < 1) return 0;
+  Carver c(nullptr, ~size_t(0) >> 1);
+  f8_buf(c, m, n, 1);
+  f8_buf(c, k, n, 128);
+  f8_buf(c, n, m, 1);
+  f8_buf(c, k, m, 1);
+  return align_up(c.used, 256) + 256;
+}
+
+extern "C" SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t ldx, int m, int n, int k, const void* w,
+                                             int w_dtype, int64_t ldw, const void* dy, int64_t dy_row, int64_t dy_col,
+                                             void* dx, void* dw, int* status, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+  if (!f8_linear_ok(dtype, ldx, m, n, k, w_dtype) || ldw < k || dy_row < 0 || dy_col < 0) return SB_ERR_ARG;
+  if (m == 0) {  // no rows: dw is a sum of none
+    if (!dw) return SB_OK;
+    return cuda_status(cudaMemsetAsync(dw, 0, static_cast<size_t>(n) * k * (w_dtype == SB_F32 ? 4 : 2),
+                                       static_cast<cudaStream_t>(stream)));
+  }
+  if (!dy || (dx && !w) || (dw && !x)) return SB_ERR_ARG;
+  Carver c(workspace, workspace_bytes);
+  const F8Buf dq = f8_buf(c, m, n, 1), wt = f8_buf(c, k, n, 128), dt = f8_buf(c, n, m, 1), xt = f8_buf(c, k, m, 1);
+  if (!workspace || c.overflow) return SB_ERR_WORKSPACE;
+#define SB_TRY(e) do { const int rc = (e); if (rc) return rc; } while (0)
+  if (dx) {  // the blocks of w^T are the transposed blocks of w: the forward pass's values
+    SB_TRY(f8_quantize(wt, w, w_dtype, k, n, 1, ldw, 128, stream));
+    SB_TRY(f8_quantize(dq, dy, dtype, m, n, dy_row, dy_col, 1, stream));
+    SB_TRY(f8_product(dq, wt, 128, m, k, n, dx, dtype, status, stream));
+  }
+  if (dw) {
+    SB_TRY(f8_quantize(dt, dy, dtype, n, m, dy_col, dy_row, 1, stream));
+    SB_TRY(f8_quantize(xt, x, dtype, k, m, 1, ldx, 1, stream));
+    SB_TRY(f8_product(dt, xt, 1, n, k, m, dw, w_dtype, status, stream));
+  }
+#undef SB_TRY
+  return SB_OK;
+}
+
 // ------------------------------------------------------------------ expert delta
 namespace sb {
 

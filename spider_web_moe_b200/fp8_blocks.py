@@ -47,20 +47,25 @@ _STATUS: dict = {}
 
 
 def _status_ptr(device) -> int | None:
-    t = _STATUS.get(device)
-    if t is None:
+    hit = _STATUS.get(device)
+    if hit is None:
         if torch.cuda.is_current_stream_capturing():
             return None  # memory of this capture's pool would not outlive the graph
-        t = _STATUS[device] = torch.zeros(1, dtype=torch.int32, device=device)
-    return t.data_ptr()
+        t = torch.zeros(1, dtype=torch.int32, device=device)
+        hit = _STATUS[device] = (t, t.data_ptr())
+    return hit[1]
 
 
 def check_status(device) -> None:
     """Raise if a kernel of this module recorded an error on ``device`` (a
     bounded wait ran out); synchronises."""
-    t = _STATUS.get(torch.device(device))
-    if t is not None and int(t.item()):
-        raise L.SpiderB200Error(L.SB_ERR_DEVICE_STATUS, f"fp8_blocks: device status 0x{int(t.item()):x}")
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
+    hit = _STATUS.get(device)
+    word = int(hit[0].item()) if hit is not None else 0
+    if word:
+        raise L.SpiderB200Error(L.SB_ERR_DEVICE_STATUS, f"fp8_blocks: device status 0x{word:x}")
 
 
 def _finish(rc: int, where: str, device) -> None:
@@ -153,8 +158,7 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> Fp8BlockTensor:
             q=q.data_ptr(), ldq=-(-c // 16) * 16, q_batch=q.stride(0) if three else 0,
             scale=scale.data_ptr(), scale_row=scale.stride(-2), scale_col=scale.stride(-1),
             scale_batch=scale.stride(0) if three else 0)
-        with torch.cuda.device(x.device):
-            rc = L.load().sb_fp8_quantize_blocks(C.byref(a), torch.cuda.current_stream(x.device).cuda_stream)
+        rc = L.on_device(x.device, lambda stream: L.load().sb_fp8_quantize_blocks(C.byref(a), stream))
         L.check(rc, "sb_fp8_quantize_blocks")
     return Fp8BlockTensor(q, scale, block_rows)
 
@@ -192,10 +196,41 @@ def fp8_block_matmul(a: Fp8BlockTensor, b: Fp8BlockTensor, out_dtype: torch.dtyp
         a_scale_block=a.scale.stride(1), b=b.q.data_ptr(), ldb=b.pitch, b_scale=b.scale.data_ptr(),
         b_scale_row=b.scale.stride(0), b_scale_block=b.scale.stride(1), b_block_rows=b.block_rows,
         out=out.data_ptr(), ldo=out.stride(0) if m > 1 else n, status=_status_ptr(out.device))
-    with torch.cuda.device(out.device):
-        rc = L.load().sb_fp8_matmul(C.byref(args), torch.cuda.current_stream(out.device).cuda_stream)
+    rc = L.on_device(out.device, lambda stream: L.load().sb_fp8_matmul(C.byref(args), stream))
     _finish(rc, "sb_fp8_matmul", out.device)
     return out
+
+
+def _unit_cols(t: torch.Tensor) -> torch.Tensor:
+    """t [R, C] with unit column stride and rows that do not overlap (a copy only if it has not)."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _linear(x, weight, packed):
+    """y [M, N] for x [M, K] in one library call."""
+    x = _unit_cols(x)
+    m, k = x.shape
+    dev = x.device
+    if packed is not None:
+        n, w, wcode, ldw, s = packed.q.shape[0], packed.q, L.SB_BF16, packed.pitch, packed.scale
+        sptr, srow, scol = s.data_ptr(), s.stride(0), s.stride(1)
+    else:
+        w = _unit_cols(weight)
+        n, wcode, ldw = w.shape[0], _DTYPES[w.dtype], max(w.stride(0), k)
+        sptr, srow, scol = None, 0, 0
+    y = torch.empty((m, n), dtype=x.dtype, device=dev)
+    if m == 0 or n == 0:
+        return y
+    if k == 0:
+        return y.zero_()
+    lib = L.load()
+    nbytes = lib.sb_fp8_linear_workspace_bytes(m, n, k, packed is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    rc = L.on_device(dev, lambda stream: lib.sb_fp8_linear(
+        x.data_ptr(), _DTYPES[x.dtype], max(x.stride(0), k), m, n, k, w.data_ptr(), wcode, ldw, sptr, srow, scol,
+        y.data_ptr(), _status_ptr(dev), ws.data_ptr(), nbytes, stream))
+    _finish(rc, "sb_fp8_linear", dev)
+    return y
 
 
 class _Fp8Linear(torch.autograd.Function):
@@ -206,20 +241,29 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, packed):
         ctx.packed = packed
         ctx.save_for_backward(x, weight)
-        w = packed if packed is not None else quantize_fp8_blocks(weight, BLOCK)
-        return fp8_block_matmul(quantize_fp8_blocks(x), w, x.dtype)
+        return _linear(x, weight, packed)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            # the blocks of w^T are the transposed blocks of w: the forward pass's values
-            wt = ctx.packed.transpose() if ctx.packed is not None else quantize_fp8_blocks(weight.t(), BLOCK)
-            dx = fp8_block_matmul(quantize_fp8_blocks(dy), wt, x.dtype)
-        if ctx.needs_input_grad[1]:
-            dw = fp8_block_matmul(quantize_fp8_blocks(dy.t()), quantize_fp8_blocks(x.t()), weight.dtype)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if ctx.packed is not None:
+            return fp8_block_matmul(quantize_fp8_blocks(dy), ctx.packed.transpose(), x.dtype), None, None
+        (m, k), n = x.shape, weight.shape[0]
+        dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty((n, k), dtype=weight.dtype, device=x.device) if need_w else None
+        if n == 0 or k == 0:
+            return (dx.zero_() if need_x else None), dw, None
+        xc, wc = _unit_cols(x), _unit_cols(weight)
+        lib = L.load()
+        nbytes = lib.sb_fp8_linear_backward_workspace_bytes(m, n, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        rc = L.on_device(x.device, lambda stream: lib.sb_fp8_linear_backward(
+            xc.data_ptr(), _DTYPES[xc.dtype], max(xc.stride(0), k), m, n, k, wc.data_ptr(), _DTYPES[wc.dtype],
+            max(wc.stride(0), k), dy.data_ptr(), dy.stride(0), dy.stride(1), L.ptr(dx), L.ptr(dw),
+            _status_ptr(x.device), ws.data_ptr(), nbytes, stream))
+        _finish(rc, "sb_fp8_linear_backward", x.device)
         return dx, dw, None
 
 
@@ -232,24 +276,23 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
     ties their gradients to the stream those were built on."""
     _dtype_code(x, "fp8_block_linear input")
     packed = weight if isinstance(weight, Fp8BlockTensor) else None
-    shape = tuple(weight.shape)
+    w = weight if packed is None else packed.q
+    shape = w.shape
     if len(shape) != 2 or x.dim() < 1 or x.shape[-1] != shape[1]:
-        raise ValueError(f"fp8_block_linear needs x [..., K] and weight [N, K], got {tuple(x.shape)} and {shape}")
-    if (packed.q if packed is not None else weight).device != x.device:
+        raise ValueError(f"fp8_block_linear needs x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(shape)}")
+    if w.device != x.device:
         raise ValueError("x and weight must be on one device")
-    if packed is not None and packed.block_rows != BLOCK:
-        raise ValueError("packed weights need 128 x 128 blocks")
     if packed is None:
         _dtype_code(weight, "fp8_block_linear weight")
+    elif packed.block_rows != BLOCK:
+        raise ValueError("packed weights need 128 x 128 blocks")
     _need_cuda(x, "fp8_block_linear")
-    x2 = x.reshape(-1, shape[1])
-    needs = torch.is_grad_enabled() and (x.requires_grad or (packed is None and weight.requires_grad))
-    if needs:
+    x2 = x if x.dim() == 2 else x.reshape(-1, shape[1])
+    if torch.is_grad_enabled() and (x.requires_grad or (packed is None and weight.requires_grad)):
         y = _Fp8Linear.apply(x2, None if packed is not None else weight, packed)
     else:
-        w = packed if packed is not None else quantize_fp8_blocks(weight, BLOCK)
-        y = fp8_block_matmul(quantize_fp8_blocks(x2), w, x.dtype)
-    return y.view(*x.shape[:-1], shape[0])
+        y = _linear(x2, weight, packed)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], shape[0])
 
 
 class Fp8BlockExperts:
@@ -306,6 +349,7 @@ class Fp8BlockExperts:
             b_up=L.ptr(self.b_up), w_gate=g.q.data_ptr() if g is not None else None,
             s_gate=g.scale.data_ptr() if g is not None else None, b_gate=L.ptr(self.b_gate),
             w_down=self.w_down.q.data_ptr(), s_down=self.w_down.scale.data_ptr(), b_down=L.ptr(self.b_down))
+        self._ref = C.byref(self._c)
 
     def weight_bytes(self) -> int:
         ts = [t for w in (self.w_up, self.w_down, self.w_gate) if w is not None for t in (w.q, w.scale)]
@@ -316,27 +360,27 @@ class Fp8BlockExperts:
         """Weighted sum of the routed experts' outputs [n, H] for messages [n, H],
         experts restricted to ``e % world == rank``."""
         lib = L.load()
+        dev = self.device
         code = _dtype_code(messages, "messages")
         out_dtype = messages.dtype if out_dtype is None else out_dtype
         n, k = top_indices.shape
-        x = messages if messages.stride(1) == 1 and messages.stride(0) >= self.hidden else messages.contiguous()
+        x = _unit_cols(messages)
         idx = top_indices
         if world > 1:
             idx = torch.where(idx % world == rank, idx, -1)
         idx = idx.to(torch.int32).contiguous()
         w = top_weights.to(torch.float32).contiguous()
-        out = torch.empty((n, -(-self.hidden // 4) * 4), dtype=out_dtype, device=self.device)
-        nbytes = lib.sb_fp8_expert_delta_workspace_bytes(C.byref(self._c), n, k)
+        cols = -(-self.hidden // 4) * 4
+        out = torch.empty((n, cols), dtype=out_dtype, device=dev)
+        nbytes = lib.sb_fp8_expert_delta_workspace_bytes(self._ref, n, k)
         if nbytes == 0:
             raise L.SpiderB200Error(L.SB_ERR_ARG, "sb_fp8_expert_delta_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        with torch.cuda.device(self.device):
-            rc = lib.sb_fp8_expert_delta(C.byref(self._c), x.data_ptr(), code, max(x.stride(0), self.hidden),
-                                         idx.data_ptr(), w.data_ptr(), n, k, out.data_ptr(), _DTYPES[out_dtype],
-                                         _status_ptr(self.device), ws.data_ptr(), ws.numel(),
-                                         torch.cuda.current_stream(self.device).cuda_stream)
-        _finish(rc, "sb_fp8_expert_delta", self.device)
-        return out[:, :self.hidden]
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = L.on_device(dev, lambda stream: lib.sb_fp8_expert_delta(
+            self._ref, x.data_ptr(), code, max(x.stride(0), self.hidden), idx.data_ptr(), w.data_ptr(), n, k,
+            out.data_ptr(), _DTYPES[out_dtype], _status_ptr(dev), ws.data_ptr(), nbytes, stream))
+        _finish(rc, "sb_fp8_expert_delta", dev)
+        return out if cols == self.hidden else out[:, :self.hidden]
 
 
 def fp8_expert_delta(messages, top_indices, top_weights, experts: Fp8BlockExperts,

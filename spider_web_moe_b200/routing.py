@@ -30,7 +30,7 @@ def _dtype_code(dtype: torch.dtype) -> int:
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """[..., E] as [n, E] with unit column stride (a copy only if there is no such view)."""
-    x = logits.reshape(-1, logits.shape[-1])
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
 
 
@@ -39,12 +39,12 @@ def _launch(logits, top_k, score, bias, num_groups, topk_groups, group_top, reno
     n, e = x.shape
     idx = torch.empty((n, top_k), dtype=torch.int32, device=x.device)
     w = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = L.load().sb_route_experts(x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n, e, top_k, score,
-                                       L.ptr(bias), num_groups, topk_groups, group_top, int(renormalize),
-                                       float(scale), idx.data_ptr(), w.data_ptr(),
-                                       torch.cuda.current_stream(x.device).cuda_stream)
+    rc = L.on_device(x.device, lambda stream: L.load().sb_route_experts(
+        x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n, e, top_k, score, L.ptr(bias), num_groups,
+        topk_groups, group_top, renormalize, scale, idx.data_ptr(), w.data_ptr(), stream))
     L.check(rc, "sb_route_experts")
+    if logits.dim() == 2:
+        return idx, w
     lead = logits.shape[:-1]
     return idx.view(*lead, top_k), w.view(*lead, top_k)
 
@@ -56,11 +56,14 @@ class _RouteExperts(torch.autograd.Function):
         ctx.save_for_backward(logits, idx, bias)
         ctx.args = (score, renormalize, scale)
         ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
         return idx, w
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, grad_w):
+        if grad_w is None:
+            return (None,) * 9
         logits, idx, bias = ctx.saved_tensors
         score, renormalize, scale = ctx.args
         x = _rows(logits)
@@ -68,11 +71,9 @@ class _RouteExperts(torch.autograd.Function):
         k = idx.shape[-1]
         g = grad_w.reshape(n, k).to(torch.float32).contiguous()
         dl = torch.empty((n, e), dtype=x.dtype, device=x.device)
-        with torch.cuda.device(x.device):
-            rc = L.load().sb_route_experts_backward(x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n, e, k,
-                                                    score, L.ptr(bias), int(renormalize), float(scale),
-                                                    idx.data_ptr(), g.data_ptr(), dl.data_ptr(), e,
-                                                    torch.cuda.current_stream(x.device).cuda_stream)
+        rc = L.on_device(x.device, lambda stream: L.load().sb_route_experts_backward(
+            x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n, e, k, score, L.ptr(bias), renormalize, scale,
+            idx.data_ptr(), g.data_ptr(), dl.data_ptr(), e, stream))
         L.check(rc, "sb_route_experts_backward")
         return dl.view(logits.shape), None, None, None, None, None, None, None, None
 
@@ -115,11 +116,12 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     if bias is not None:
         if bias.shape != (e,) or bias.device != logits.device:
             raise ValueError("bias must be [E] on the logits' device")
-        bias = bias.detach().to(torch.float32).contiguous()
+        if bias.dtype != torch.float32 or bias.requires_grad or not bias.is_contiguous():
+            bias = bias.detach().to(torch.float32).contiguous()
     if not logits.is_cuda:
         raise RuntimeError("spider_b200 route_experts runs on CUDA tensors only")
     args = (int(top_k), SCORES[score], int(num_groups), int(topk_groups), GROUP_SCORES[group_score],
-            bool(renormalize), float(scale))
+            int(bool(renormalize)), float(scale))
     if torch.is_grad_enabled() and logits.requires_grad:
         return _RouteExperts.apply(logits, bias, *args)
     return _launch(logits.detach(), args[0], args[1], bias, *args[2:])

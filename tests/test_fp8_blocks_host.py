@@ -143,3 +143,16 @@ def test_c_abi_refuses_before_any_launch():
         setattr(e, f, p)
     assert call(p, need - 256) == L.SB_ERR_WORKSPACE
     assert call(None, need) == L.SB_ERR_WORKSPACE
+
+    assert lib.sb_fp8_linear_workspace_bytes(4, 8, 0, 0) == 0
+    need = lib.sb_fp8_linear_workspace_bytes(4, 8, 32, 0)
+    assert need > lib.sb_fp8_linear_workspace_bytes(4, 8, 32, 1) > 0
+    lin = lambda x=p, dt=0, ld=32, wd=0, ldw=32, w=p, ws=p, n=need: lib.sb_fp8_linear(  # noqa: E731
+        x, dt, ld, 4, 8, 32, w, wd, ldw, None, 0, 0, p, None, ws, n, None)
+    assert lin(x=None) == lin(dt=2) == lin(ld=31) == lin(wd=3) == lin(ldw=31) == lin(w=None) == L.SB_ERR_ARG
+    assert lin(ws=None) == lin(n=64) == L.SB_ERR_WORKSPACE
+    need = lib.sb_fp8_linear_backward_workspace_bytes(4, 8, 32)
+    back = lambda x=p, w=p, dy=p, dr=8, n=need: lib.sb_fp8_linear_backward(  # noqa: E731
+        x, 0, 32, 4, 8, 32, w, 0, 32, dy, dr, 1, p, p, None, p, n, None)
+    assert back(x=None) == back(w=None) == back(dy=None) == back(dr=-1) == L.SB_ERR_ARG
+    assert back(n=64) == L.SB_ERR_WORKSPACE
