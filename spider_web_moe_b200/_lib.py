@@ -238,12 +238,12 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
-def on_device(device, call):
-    """call(raw stream pointer of the device's current stream), with that device
+def on_device(device, fn, *args) -> int:
+    """fn(*args, raw pointer of the device's current stream) with that device
     current (the library launches on the current device)."""
     index = device.index
-    stream = torch.cuda.current_stream(index).cuda_stream
-    if torch.cuda.current_device() == index:
-        return call(stream)
+    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream without the Stream object
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, stream)
     with torch.cuda.device(index):
-        return call(stream)
+        return fn(*args, stream)

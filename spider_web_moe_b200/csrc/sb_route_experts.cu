@@ -63,136 +63,189 @@ struct RouteParams {
   float* top_w;
 };
 
-// Which of a token's candidates are taken.  key[v] is the order key of expert
-// lane + 32 v (0: not a candidate); returns, in lane j < K, the j-th expert.
-// With kCheck, *close is set when an expert was taken while another one that is
-// not exactly equal to it (same logit, same bias) lay within the fp32 error.
-template <int V, bool kCheck, typename Key>
-SB_DEVINL int select_top(Key (&key)[V], const float (&l)[V], const float (&b)[V], int K, int lane, float tol,
-                         bool* close) {
+// Lane i holds the V experts [i V, i V + V): a lower lane means lower ids, so the
+// lowest lane that holds the largest choice has the expert that wins a tie.
+
+// A token's logits (-inf past E).  kVec: rows are aligned for whole-lane loads
+// and E is a multiple of V.
+template <typename T, int V, bool kVec>
+SB_DEVINL void load_logits(const T* __restrict__ row, int E, int lane, float (&l)[V]) {
+  const int e0 = lane * V;
+  if constexpr (kVec) {
+    constexpr int kBytes = V * sizeof(T);
+    constexpr int kWords = kBytes / 4;
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+    if (e0 < E) {
+      if constexpr (kBytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(row + e0) + 4 * i);
+          w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+        }
+      } else if constexpr (kBytes == 8) {
+        const uint2 u = *reinterpret_cast<const uint2*>(row + e0);
+        w[0] = u.x; w[1] = u.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(row + e0);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float x = sizeof(T) == 4 ? __uint_as_float(w[v])
+                                     : __uint_as_float(v & 1 ? w[v / 2] & 0xffff0000u : w[v / 2] << 16);
+      l[v] = e0 < E ? x : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) l[v] = e0 + v < E ? to_f32<T>(row[e0 + v]) : -INFINITY;
+  }
+}
+
+// The K largest keys (0: no candidate): lane j < K returns the j-th expert and
+// its key.  Taken keys are zeroed.
+template <int V, typename Key>
+SB_DEVINL int select_top(Key (&key)[V], int K, int lane, Key* mine_key) {
   int mine = 0;
-  bool near = false;
   for (int j = 0; j < K; ++j) {
     Key best = key[0];
 #pragma unroll
     for (int v = 1; v < V; ++v) best = key[v] > best ? key[v] : best;
     const Key top = warp_max_key(best);
-    uint32_t e = 0xffffffffu;
+    const int winner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+    int at = 0;  // the lowest expert of this lane that has the largest key
 #pragma unroll
     for (int v = V - 1; v >= 0; --v)
-      if (key[v] == top) e = lane + 32 * v;
-    e = __reduce_min_sync(0xffffffffu, e);
-    if (kCheck) {
-      float cl = 0.f, cb = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (lane + 32 * v == static_cast<int>(e)) { cl = l[v]; cb = b[v]; }
-      cl = __shfl_sync(0xffffffffu, cl, e & 31);
-      cb = __shfl_sync(0xffffffffu, cb, e & 31);
-      const float c = static_cast<float>(key_value(top));
-      const Key limit = order_key(c - (tol + fabsf(c) * 0x1p-22f));
-#pragma unroll
-      for (int v = 0; v < V; ++v) near |= key[v] >= limit && key[v] != 0 && (l[v] != cl || b[v] != cb);
-    }
-    if (lane == j) mine = static_cast<int>(e);
+      if (key[v] == top) at = v;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (lane + 32 * v == static_cast<int>(e)) key[v] = 0;
+      if (lane == winner && v == at) key[v] = 0;
+    const int e = __shfl_sync(0xffffffffu, lane * V + at, winner);
+    if (lane == j) {
+      mine = e;
+      *mine_key = top;
+    }
   }
-  if (kCheck) *close |= __any_sync(0xffffffffu, near);
   return mine;
 }
 
-// Drops the candidates outside the best topk_groups groups.  ch: the warp's
-// keys of all experts in shared memory.
-template <int V, bool kCheck, typename Key>
-SB_DEVINL void keep_groups(Key (&key)[V], Key* ch, const RouteParams& p, int lane, float tol, bool* close) {
+// Drops the candidates outside the best topk_groups groups; returns whether a
+// group left out came within `tol` of the last one kept.  `ch`: room for the
+// warp's keys of all experts in shared memory, for groups that are not a power
+// of two of whole lanes.
+template <int V, typename Key>
+SB_DEVINL bool keep_groups(Key (&key)[V], Key* ch, const RouteParams& p, int lane, float tol) {
   using Val = decltype(key_value(Key(0)));
-  const int per = p.E / p.groups;
+  const int per = p.E / p.groups, lanes = per / V;
+  const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
+  Key k1 = 0, k2 = 0;
+  if (whole) {
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (lane + 32 * v < p.E) ch[lane + 32 * v] = key[v];
-  __syncwarp();
-  Key gk = 0;
-  if (lane < p.groups) {
-    Key k1 = 0, k2 = 0;
-    for (int i = 0; i < per; ++i) {
+    for (int v = 0; v < V; ++v) {
+      const Key lo = key[v] < k1 ? key[v] : k1;
+      k1 = key[v] > k1 ? key[v] : k1;
+      k2 = lo > k2 ? lo : k2;
+    }
+    for (int o = 1; o < lanes; o <<= 1) {
+      const Key o1 = __shfl_xor_sync(0xffffffffu, k1, o), o2 = __shfl_xor_sync(0xffffffffu, k2, o);
+      const Key lo = o1 < k1 ? o1 : k1;
+      k1 = o1 > k1 ? o1 : k1;
+      k2 = o2 > k2 ? o2 : k2;
+      k2 = lo > k2 ? lo : k2;
+    }
+    const int src = lane * lanes < 32 ? lane * lanes : 0;  // from here lane g holds group g
+    k1 = __shfl_sync(0xffffffffu, k1, src);
+    k2 = __shfl_sync(0xffffffffu, k2, src);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (lane * V + v < p.E) ch[lane * V + v] = key[v];
+    __syncwarp();
+    for (int i = 0; lane < p.groups && i < per; ++i) {
       const Key k = ch[lane * per + i];
       if (k > k1) { k2 = k1; k1 = k; } else if (k > k2) k2 = k;
     }
-    Val gs = key_value(k1);
-    if (p.group_top == 2 && per > 1) gs += key_value(k2);
-    gk = order_key(gs);
+    __syncwarp();
   }
-  __syncwarp();
-  uint32_t kept = 0;
-  Key top = 0;
-  for (int j = 0; j < p.topk_groups; ++j) {
-    top = warp_max_key(gk);
-    const int g = __ffs(__ballot_sync(0xffffffffu, gk == top)) - 1;
-    kept |= 1u << g;
-    if (lane == g) gk = 0;
+  Val gs = key_value(k1);
+  if (p.group_top == 2 && per > 1) gs += key_value(k2);
+  const Key gk = lane < p.groups ? order_key(gs) : 0;
+  int rank = 0;  // groups ahead of this lane's
+  for (int g = 0; g < p.groups; ++g) {
+    const Key o = __shfl_sync(0xffffffffu, gk, g);
+    rank += (o > gk || (o == gk && g < lane)) ? 1 : 0;
   }
-  if (kCheck) {  // a group left out within the error of the last one kept
-    const float c = static_cast<float>(key_value(top));
-    *close |= __any_sync(0xffffffffu, gk != 0 && gk >= order_key(c - (2.f * tol + fabsf(c) * 0x1p-21f)));
-  }
+  const bool in = lane < p.groups && rank < p.topk_groups;
+  const uint32_t kept = __ballot_sync(0xffffffffu, in);
+  const int last = __ffs(__ballot_sync(0xffffffffu, lane < p.groups && rank == p.topk_groups - 1)) - 1;
+  const float c = static_cast<float>(__shfl_sync(0xffffffffu, gs, last));
+  const bool near = lane < p.groups && !in && gk >= order_key(static_cast<Val>(c - (tol + fabsf(c) * 0x1p-21f)));
+  if (whole) {
+    const bool mine = (kept >> (lane / lanes & 31)) & 1u;  // lanes past the last expert hold no keys
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    if (e < p.E && !((kept >> (e / per)) & 1u)) key[v] = 0;
+    for (int v = 0; v < V; ++v) key[v] = mine ? key[v] : 0;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = lane * V + v;
+      if (e < p.E && !((kept >> (e / per)) & 1u)) key[v] = 0;
+    }
   }
+  return __any_sync(0xffffffffu, near);
 }
 
-// The selection from fp64 scores.
-template <int V>
-__device__ __noinline__ int select_f64(const float (&l)[V], const float (&b)[V], const RouteParams& p,
-                                       unsigned long long* ch, int lane) {
-  double m = -INFINITY, sum = 0.0;
+// The selection from fp64 scores; rare, so it reads the logits again rather
+// than have the caller keep them.
+template <typename T, int V>
+__device__ __noinline__ int select_f64(const T* __restrict__ row, const RouteParams& p, unsigned long long* ch, int lane) {
+  double m = 0.0, sum = 0.0;
   if (p.score == SB_SCORE_SOFTMAX) {
     float mf = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < V; ++v) mf = fmaxf(mf, l[v]);
-    m = warp_max(mf);
-#pragma unroll
     for (int v = 0; v < V; ++v)
-      if (l[v] > -INFINITY) sum += exp(static_cast<double>(l[v]) - m);
+      if (lane * V + v < p.E) mf = fmaxf(mf, to_f32<T>(row[lane * V + v]));
+    m = warp_max(mf);
+    for (int v = 0; v < V; ++v) {
+      const float x = lane * V + v < p.E ? to_f32<T>(row[lane * V + v]) : -INFINITY;
+      if (x != -INFINITY) sum += exp(static_cast<double>(x) - m);
+    }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   unsigned long long key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const double x = l[v];
-    const double s = p.score == SB_SCORE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x));
-    const double c = (l[v] == -INFINITY || b[v] == -INFINITY) ? -INFINITY : s + static_cast<double>(b[v]);
-    key[v] = lane + 32 * v < p.E ? order_key(c) : 0;
+    const int e = lane * V + v;
+    key[v] = 0;
+    if (e < p.E) {
+      const float l = to_f32<T>(row[e]), b = p.bias ? p.bias[e] : 0.f;
+      const double x = l;
+      const double s = p.score == SB_SCORE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x));
+      key[v] = order_key((l == -INFINITY || b == -INFINITY) ? -INFINITY : s + static_cast<double>(b));
+    }
   }
-  bool unused = false;
-  if (p.topk_groups < p.groups) keep_groups<V, false>(key, ch, p, lane, 0.f, &unused);
-  return select_top<V, false>(key, l, b, p.K, lane, 0.f, &unused);
+  if (p.topk_groups < p.groups) keep_groups<V>(key, ch, p, lane, 0.f);
+  unsigned long long unused;
+  return select_top<V>(key, p.K, lane, &unused);
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict__ logits, const RouteParams p) {
+template <typename T, int V, bool kVec>
+__global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict__ logits, const __grid_constant__ RouteParams p) {
   extern __shared__ __align__(16) uint8_t route_smem[];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp;
   if (t >= p.n) return;
-  unsigned long long* ch64 = reinterpret_cast<unsigned long long*>(route_smem) + static_cast<size_t>(warp) * p.E;
-  float* s_sm = reinterpret_cast<float*>(ch64);
+  unsigned long long* ch = reinterpret_cast<unsigned long long*>(route_smem) + static_cast<size_t>(warp) * p.E;
   const T* row = logits + t * p.ld;
-  float l[V], b[V], s[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    l[v] = e < p.E ? to_f32<T>(row[e]) : -INFINITY;
-    b[v] = e < p.E && p.bias ? p.bias[e] : 0.f;
-  }
-  float sum = 0.f;
-  if (p.score == SB_SCORE_SOFTMAX) {
-    float m = -INFINITY;
+  const bool softmax = p.score == SB_SCORE_SOFTMAX;
+  const bool grouped = p.topk_groups < p.groups;
+  // without a bias the choices are monotonic in the logits, unless two are added
+  const bool by_logit = !p.bias && !(grouped && p.group_top == 2);
+  float l[V];
+  load_logits<T, V, kVec>(row, p.E, lane, l);
+  float m = -INFINITY, sum = 0.f, inv = 0.f, s[V];
+  if (softmax) {
 #pragma unroll
     for (int v = 0; v < V; ++v) m = fmaxf(m, l[v]);
     m = warp_max(m);
@@ -202,45 +255,65 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
       sum += s[v];
     }
     sum = warp_sum(sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] *= inv;
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = 1.f / (1.f + expf(-l[v]));
+    inv = sum == 0.f ? 0.f : 1.f / sum;
   }
-  const bool grouped = p.topk_groups < p.groups;
-  const bool by_logit = !p.bias && !(grouped && p.group_top == 2);
   uint32_t key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    // a NaN anywhere in a softmax row makes every score of the row NaN
-    const float c = by_logit ? l[v] + 0.f * sum : ((l[v] == -INFINITY || b[v] == -INFINITY) ? -INFINITY : s[v] + b[v]);
-    key[v] = lane + 32 * v < p.E ? order_key(c) : 0;
+    const int e = lane * V + v;
+    float c;
+    if (by_logit) {
+      c = l[v] + 0.f * sum;  // a NaN anywhere in a softmax row makes every score of the row NaN
+    } else {
+      const float b = e < p.E && p.bias ? p.bias[e] : 0.f;
+      // the fast sigmoid: (1.5 |x| + 4) s (1 - s) 2^-23 off, below 2^-21
+      const float sc = softmax ? s[v] * inv : __fdividef(1.f, 1.f + __expf(-l[v]));
+      c = (l[v] == -INFINITY || b == -INFINITY) ? -INFINITY : sc + b;
+    }
+    key[v] = e < p.E ? order_key(c) : 0;
   }
   // fp32 error of a score: exp of a rounded difference (|x| e^-|x| 2^-24 <=
   // 0.37 2^-24), 2 ulp of expf, the sum and the division, all below 2^-20 in
   // all; two of them may differ by 2^-19.
   constexpr float kTol = 0x1p-19f;
   bool close = false;
-  int mine;
-  if (by_logit) {
-    if (grouped) keep_groups<V, false>(key, reinterpret_cast<uint32_t*>(ch64), p, lane, 0.f, &close);
-    mine = select_top<V, false>(key, l, b, p.K, lane, 0.f, &close);
-  } else {
-    if (grouped) keep_groups<V, true>(key, reinterpret_cast<uint32_t*>(ch64), p, lane, kTol, &close);
-    mine = select_top<V, true>(key, l, b, p.K, lane, kTol, &close);
-    if (close) mine = select_f64<V>(l, b, p, ch64, lane);
-  }
-  __syncwarp();
+  if (grouped) close = keep_groups<V>(key, reinterpret_cast<uint32_t*>(ch), p, lane, 2.f * kTol);
+  uint32_t mine_key = 0;
+  int mine = select_top<V>(key, p.K, lane, &mine_key);
+  float ls = lane < p.K ? to_f32<T>(row[mine]) : -INFINITY;
+  float bs = lane < p.K && p.bias ? p.bias[mine] : 0.f;
+  if (!by_logit) {
+    // Did a decision hang on a gap that fp32 does not resolve?  Between one taken
+    // expert and the next, or between the last taken and one left out, unless
+    // the two are exactly equal (same logit, same bias).  (If such a gap lies
+    // further up, the experts between are exactly equal to its upper end.)
+    const float c = key_value(mine_key);
+    const float pc = __shfl_up_sync(0xffffffffu, c, 1), pl = __shfl_up_sync(0xffffffffu, ls, 1),
+                pb = __shfl_up_sync(0xffffffffu, bs, 1);
+    if (lane > 0 && lane < p.K && pc - c <= kTol + fabsf(pc) * 0x1p-22f && (pl != ls || pb != bs)) close = true;
+    const float lc = __shfl_sync(0xffffffffu, c, p.K - 1);
+    const uint32_t limit = order_key(lc - (kTol + fabsf(lc) * 0x1p-22f));
+    bool near = false;
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (lane + 32 * v < p.E) s_sm[lane + 32 * v] = (l[v] == -INFINITY || b[v] == -INFINITY) ? 0.f : s[v];
-  __syncwarp();
-  float w = lane < p.K ? s_sm[mine] : 0.f;
+    for (int v = 0; v < V; ++v) near |= key[v] >= limit;
+    if (__any_sync(0xffffffffu, near)) {
+      const float ll = __shfl_sync(0xffffffffu, ls, p.K - 1), lb = __shfl_sync(0xffffffffu, bs, p.K - 1);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (key[v] >= limit && key[v] != 0 && (l[v] != ll || (p.bias ? p.bias[lane * V + v] : 0.f) != lb)) close = true;
+    }
+    if (__any_sync(0xffffffffu, close)) {
+      mine = select_f64<T, V>(row, p, ch, lane);
+      ls = lane < p.K ? to_f32<T>(row[mine]) : -INFINITY;
+      bs = lane < p.K && p.bias ? p.bias[mine] : 0.f;
+    }
+  }
+  float w = 0.f;
+  if (lane < p.K && ls != -INFINITY && bs != -INFINITY)
+    w = softmax ? expf(ls - m) * inv : 1.f / (1.f + expf(-ls));
   if (p.renorm) {
-    const float sum = warp_sum(w);
-    w /= sum < 1e-9f ? 1e-9f : sum;  // not fmaxf, which would hide a NaN
+    const float total = warp_sum(w);
+    w /= total < 1e-9f ? 1e-9f : total;  // not fmaxf, which would hide a NaN
   }
   if (lane < p.K) {
     p.top_idx[t * p.K + lane] = mine;
@@ -252,9 +325,9 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
 //   ds_j = scale (g_j - (sum_k g_k s_k) / D) / D   (renormalised, D = sum s)
 //   ds_j = scale g_j / D'                          (D' = 1, or the floor 1e-9)
 //   softmax: dl_i = s_i (ds_i - sum_k ds_k s_k);  sigmoid: dl_j = ds_j s_j (1 - s_j)
-template <typename T, int V>
+template <typename T, int V, bool kVec>
 __global__ void __launch_bounds__(256)
-route_experts_backward_kernel(const T* __restrict__ logits, const RouteParams p, const float* __restrict__ gw,
+route_experts_backward_kernel(const T* __restrict__ logits, const __grid_constant__ RouteParams p, const float* __restrict__ gw,
                               T* __restrict__ dl, int64_t ldd) {
   pdl_wait();
   pdl_trigger();
@@ -262,27 +335,23 @@ route_experts_backward_kernel(const T* __restrict__ logits, const RouteParams p,
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp;
   if (t >= p.n) return;
   const T* row = logits + t * p.ld;
-  float l[V], s[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    l[v] = e < p.E ? to_f32<T>(row[e]) : -INFINITY;
-  }
   const int sel = lane < p.K ? p.top_idx[t * p.K + lane] : -1;
   const bool in_range = sel >= 0 && sel < p.E;
   const float g = in_range ? gw[t * p.K + lane] : 0.f;
   const float lsel = in_range ? to_f32<T>(row[sel]) : -INFINITY;
   const bool masked = lsel == -INFINITY || (p.bias && in_range && p.bias[sel] == -INFINITY);
+  float s[V];
   float ssel;
   if (p.score == SB_SCORE_SOFTMAX) {
+    load_logits<T, V, kVec>(row, p.E, lane, s);
     float m = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < V; ++v) m = fmaxf(m, l[v]);
+    for (int v = 0; v < V; ++v) m = fmaxf(m, s[v]);
     m = warp_max(m);
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      s[v] = l[v] == -INFINITY ? 0.f : expf(l[v] - m);
+      s[v] = s[v] == -INFINITY ? 0.f : expf(s[v] - m);
       sum += s[v];
     }
     sum = warp_sum(sum);
@@ -302,26 +371,45 @@ route_experts_backward_kernel(const T* __restrict__ logits, const RouteParams p,
     ds = p.scale * (sum < 1e-9f ? g : g - dot / d) / d;
   }
   if (masked) ds = 0.f;
-  float add = ds * ssel * (1.f - ssel);  // sigmoid
-  float dot = 0.f;
-  if (p.score == SB_SCORE_SOFTMAX) {
-    dot = warp_sum(ds * ssel);
-    add = ds;
-  }
   float dv[V];
+  float add;
+  if (p.score == SB_SCORE_SOFTMAX) {
+    const float dot = warp_sum(ds * ssel);
 #pragma unroll
-  for (int v = 0; v < V; ++v) dv[v] = 0.f;
+    for (int v = 0; v < V; ++v) dv[v] = -dot;
+    add = ds;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      dv[v] = 0.f;
+      s[v] = 1.f;
+    }
+    add = ds * ssel * (1.f - ssel);
+  }
   for (int j = 0; j < p.K; ++j) {
-    const int e = __shfl_sync(0xffffffffu, sel, j);
+    const int at = __shfl_sync(0xffffffffu, sel, j) - lane * V;
     const float a = __shfl_sync(0xffffffffu, add, j);
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (lane + 32 * v == e) dv[v] = a;
+      if (v == at) dv[v] += a;
   }
+  T* out = dl + t * ldd + lane * V;
+  if constexpr (kVec) {
+    if (lane * V >= p.E) return;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    if (e < p.E) dl[t * ldd + e] = from_f32<T>(p.score == SB_SCORE_SOFTMAX ? s[v] * (dv[v] - dot) : dv[v]);
+      for (int v = 0; v < V; v += 4)
+        *reinterpret_cast<float4*>(out + v) =
+            make_float4(s[v] * dv[v], s[v + 1] * dv[v + 1], s[v + 2] * dv[v + 2], s[v + 3] * dv[v + 3]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; v += 2)
+        reinterpret_cast<__nv_bfloat162*>(out)[v / 2] = __floats2bfloat162_rn(s[v] * dv[v], s[v + 1] * dv[v + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (lane * V + v < p.E) out[v] = from_f32<T>(s[v] * dv[v]);
   }
 }
 
@@ -332,20 +420,39 @@ static bool route_args_ok(int dtype, int64_t ld, int n, int E, int K, int score)
 
 static int route_warps(int E) { return E <= 256 ? 8 : 4; }
 
+// Whole-lane vector loads (and stores of the gradient): four or more experts a
+// lane, all lanes full or empty, rows on 16-byte (or, below, on lane) boundaries.
+template <typename T, int V>
+static bool route_vec(const void* base, int64_t ld, int E) {
+  constexpr int kBytes = V * sizeof(T) < 16 ? V * sizeof(T) : 16;
+  return E % V == 0 && reinterpret_cast<uintptr_t>(base) % kBytes == 0 && ld * sizeof(T) % kBytes == 0;
+}
+
 template <typename T, int V>
 static int launch_route(const void* logits, const RouteParams& p, cudaStream_t st) {
   const int warps = route_warps(p.E);
-  const size_t smem = static_cast<size_t>(warps) * p.E * 8;  // at most 4 * 1024 * 8 = 32 KB
-  return launch(route_experts_kernel<T, V>, dim3((p.n + warps - 1) / warps), dim3(warps * 32), smem, st,
-                static_cast<const T*>(logits), p);
+  // keys of the group scan: 4 bytes an expert, 8 in the fp64 selection
+  const size_t smem = p.topk_groups < p.groups ? static_cast<size_t>(warps) * p.E * 8 : 0;  // at most 32 KB
+  const dim3 grid((p.n + warps - 1) / warps), block(warps * 32);
+  if constexpr (V >= 4) {
+    if (route_vec<T, V>(logits, p.ld, p.E))
+      return launch(route_experts_kernel<T, V, true>, grid, block, smem, st, static_cast<const T*>(logits), p);
+  }
+  return launch(route_experts_kernel<T, V, false>, grid, block, smem, st, static_cast<const T*>(logits), p);
 }
 
 template <typename T, int V>
 static int launch_route_backward(const void* logits, const RouteParams& p, const float* gw, void* dl, int64_t ldd,
                                  cudaStream_t st) {
   const int warps = route_warps(p.E);
-  return launch(route_experts_backward_kernel<T, V>, dim3((p.n + warps - 1) / warps), dim3(warps * 32), 0, st,
-                static_cast<const T*>(logits), p, gw, static_cast<T*>(dl), ldd);
+  const dim3 grid((p.n + warps - 1) / warps), block(warps * 32);
+  if constexpr (V >= 4) {
+    if (route_vec<T, V>(logits, p.ld, p.E) && route_vec<T, V>(dl, ldd, p.E))
+      return launch(route_experts_backward_kernel<T, V, true>, grid, block, 0, st, static_cast<const T*>(logits), p, gw,
+                    static_cast<T*>(dl), ldd);
+  }
+  return launch(route_experts_backward_kernel<T, V, false>, grid, block, 0, st, static_cast<const T*>(logits), p, gw,
+                static_cast<T*>(dl), ldd);
 }
 
 #define SB_ROUTE_DISPATCH(FN, ...)                                              \

@@ -158,7 +158,7 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> Fp8BlockTensor:
             q=q.data_ptr(), ldq=-(-c // 16) * 16, q_batch=q.stride(0) if three else 0,
             scale=scale.data_ptr(), scale_row=scale.stride(-2), scale_col=scale.stride(-1),
             scale_batch=scale.stride(0) if three else 0)
-        rc = L.on_device(x.device, lambda stream: L.load().sb_fp8_quantize_blocks(C.byref(a), stream))
+        rc = L.on_device(x.device, L.load().sb_fp8_quantize_blocks, C.byref(a))
         L.check(rc, "sb_fp8_quantize_blocks")
     return Fp8BlockTensor(q, scale, block_rows)
 
@@ -196,7 +196,7 @@ def fp8_block_matmul(a: Fp8BlockTensor, b: Fp8BlockTensor, out_dtype: torch.dtyp
         a_scale_block=a.scale.stride(1), b=b.q.data_ptr(), ldb=b.pitch, b_scale=b.scale.data_ptr(),
         b_scale_row=b.scale.stride(0), b_scale_block=b.scale.stride(1), b_block_rows=b.block_rows,
         out=out.data_ptr(), ldo=out.stride(0) if m > 1 else n, status=_status_ptr(out.device))
-    rc = L.on_device(out.device, lambda stream: L.load().sb_fp8_matmul(C.byref(args), stream))
+    rc = L.on_device(out.device, L.load().sb_fp8_matmul, C.byref(args))
     _finish(rc, "sb_fp8_matmul", out.device)
     return out
 
@@ -226,9 +226,8 @@ def _linear(x, weight, packed):
     lib = L.load()
     nbytes = lib.sb_fp8_linear_workspace_bytes(m, n, k, packed is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    rc = L.on_device(dev, lambda stream: lib.sb_fp8_linear(
-        x.data_ptr(), _DTYPES[x.dtype], max(x.stride(0), k), m, n, k, w.data_ptr(), wcode, ldw, sptr, srow, scol,
-        y.data_ptr(), _status_ptr(dev), ws.data_ptr(), nbytes, stream))
+    rc = L.on_device(dev, lib.sb_fp8_linear, x.data_ptr(), _DTYPES[x.dtype], max(x.stride(0), k), m, n, k, w.data_ptr(),
+                     wcode, ldw, sptr, srow, scol, y.data_ptr(), _status_ptr(dev), ws.data_ptr(), nbytes)
     _finish(rc, "sb_fp8_linear", dev)
     return y
 
@@ -259,10 +258,9 @@ class _Fp8Linear(torch.autograd.Function):
         lib = L.load()
         nbytes = lib.sb_fp8_linear_backward_workspace_bytes(m, n, k)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        rc = L.on_device(x.device, lambda stream: lib.sb_fp8_linear_backward(
-            xc.data_ptr(), _DTYPES[xc.dtype], max(xc.stride(0), k), m, n, k, wc.data_ptr(), _DTYPES[wc.dtype],
-            max(wc.stride(0), k), dy.data_ptr(), dy.stride(0), dy.stride(1), L.ptr(dx), L.ptr(dw),
-            _status_ptr(x.device), ws.data_ptr(), nbytes, stream))
+        rc = L.on_device(x.device, lib.sb_fp8_linear_backward, xc.data_ptr(), _DTYPES[xc.dtype], max(xc.stride(0), k),
+                         m, n, k, wc.data_ptr(), _DTYPES[wc.dtype], max(wc.stride(0), k), dy.data_ptr(), dy.stride(0),
+                         dy.stride(1), L.ptr(dx), L.ptr(dw), _status_ptr(x.device), ws.data_ptr(), nbytes)
         _finish(rc, "sb_fp8_linear_backward", x.device)
         return dx, dw, None
 
@@ -376,9 +374,9 @@ class Fp8BlockExperts:
         if nbytes == 0:
             raise L.SpiderB200Error(L.SB_ERR_ARG, "sb_fp8_expert_delta_workspace_bytes")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        rc = L.on_device(dev, lambda stream: lib.sb_fp8_expert_delta(
-            self._ref, x.data_ptr(), code, max(x.stride(0), self.hidden), idx.data_ptr(), w.data_ptr(), n, k,
-            out.data_ptr(), _DTYPES[out_dtype], _status_ptr(dev), ws.data_ptr(), nbytes, stream))
+        rc = L.on_device(dev, lib.sb_fp8_expert_delta, self._ref, x.data_ptr(), code, max(x.stride(0), self.hidden),
+                         idx.data_ptr(), w.data_ptr(), n, k, out.data_ptr(), _DTYPES[out_dtype], _status_ptr(dev),
+                         ws.data_ptr(), nbytes)
         _finish(rc, "sb_fp8_expert_delta", dev)
         return out if cols == self.hidden else out[:, :self.hidden]
 

@@ -39,9 +39,9 @@ def _launch(logits, top_k, score, bias, num_groups, topk_groups, group_top, reno
     n, e = x.shape
     idx = torch.empty((n, top_k), dtype=torch.int32, device=x.device)
     w = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
-    rc = L.on_device(x.device, lambda stream: L.load().sb_route_experts(
-        x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n, e, top_k, score, L.ptr(bias), num_groups,
-        topk_groups, group_top, renormalize, scale, idx.data_ptr(), w.data_ptr(), stream))
+    rc = L.on_device(x.device, L.load().sb_route_experts, x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n,
+                     e, top_k, score, L.ptr(bias), num_groups, topk_groups, group_top, renormalize, scale,
+                     idx.data_ptr(), w.data_ptr())
     L.check(rc, "sb_route_experts")
     if logits.dim() == 2:
         return idx, w
@@ -71,9 +71,9 @@ class _RouteExperts(torch.autograd.Function):
         k = idx.shape[-1]
         g = grad_w.reshape(n, k).to(torch.float32).contiguous()
         dl = torch.empty((n, e), dtype=x.dtype, device=x.device)
-        rc = L.on_device(x.device, lambda stream: L.load().sb_route_experts_backward(
-            x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n, e, k, score, L.ptr(bias), renormalize, scale,
-            idx.data_ptr(), g.data_ptr(), dl.data_ptr(), e, stream))
+        rc = L.on_device(x.device, L.load().sb_route_experts_backward, x.data_ptr(), _dtype_code(x.dtype),
+                         max(x.stride(0), e), n, e, k, score, L.ptr(bias), renormalize, scale, idx.data_ptr(),
+                         g.data_ptr(), dl.data_ptr(), e)
         L.check(rc, "sb_route_experts_backward")
         return dl.view(logits.shape), None, None, None, None, None, None, None, None
 
