@@ -14,9 +14,11 @@
 // Two choices can lie closer together than fp32 resolves them (at 256 experts
 // about one token in 300), and which of them wins decides an index.  So the
 // fp32 selection also looks at the gaps next to every decision it makes; a
-// token with a gap inside the fp32 error is decided again from fp64 scores.
-// Without a bias the choices are monotonic in the logits, which decide then,
-// exactly.
+// token with a gap inside the fp32 error is decided again, exactly: from fp64
+// scores, or from the logits where the choices are monotonic in them (no bias).
+//
+// Bound by instructions, not memory: the fewest per token were found with the
+// experts of a lane sorted once, and then one warp maximum per expert taken.
 #include "sb_common.cuh"
 #include "sb_internal.h"
 
@@ -29,9 +31,8 @@ constexpr int kRouteMaxGroups = 32;
 // Order-preserving integer of a float: NaN above +inf, -0 equal to +0; every
 // value, -inf too, is above 0, which marks an expert that is not a candidate.
 SB_DEVINL uint32_t order_key(float v) {
-  if (v != v) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(v + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint(v + 0.0f);  // the sum of a NaN is the positive NaN
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 SB_DEVINL unsigned long long order_key(double v) {
   if (v != v) return ~0ull;
@@ -39,7 +40,6 @@ SB_DEVINL unsigned long long order_key(double v) {
   return (u >> 63) ? ~u : (u | (1ull << 63));
 }
 SB_DEVINL float key_value(uint32_t k) {
-  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 SB_DEVINL double key_value(unsigned long long k) {
@@ -61,6 +61,8 @@ struct RouteParams {
   float scale;
   int32_t* top_idx;
   float* top_w;
+  int per_group;    // E / groups
+  int group_shift;  // a group is 2^group_shift whole lanes of the kernel's V experts, or -1
 };
 
 // Lane i holds the V experts [i V, i V + V): a lower lane means lower ids, so the
@@ -103,16 +105,85 @@ SB_DEVINL void load_logits(const T* __restrict__ row, int E, int lane, float (&l
   }
 }
 
-// The K largest keys (0: no candidate): lane j < K returns the j-th expert and
-// its key.  Taken keys are zeroed.
-template <int V, typename Key>
-SB_DEVINL int select_top(Key (&key)[V], int K, int lane, Key* mine_key) {
+// The keys of the fast selection: the order key with its last bits replaced by
+// the expert's place in the lane, so that a lane's experts sort with one minimum
+// and one maximum per exchange, equal choices by lower id.  What the bits lose
+// is below the closeness tolerance, or caught by it.
+template <int V>
+constexpr uint32_t kPlaceMask = V - 1;
+
+SB_DEVINL float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The choice of a key without the place: not below -inf, whose last bits it took.
+SB_DEVINL float place_key_value(uint32_t k) { return key_value(max(k, 0x007fffffu)); }
+
+template <int V>
+SB_DEVINL void sort_descending(uint32_t (&k)[V]) {
+#pragma unroll
+  for (int size = 2; size <= V; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if ((i & d) == 0) {
+          const bool down = (i & size) == 0 || size == V;
+          const uint32_t a = k[i], b = k[i | d];
+          k[i] = down ? max(a, b) : min(a, b);
+          k[i | d] = down ? min(a, b) : max(a, b);
+        }
+}
+
+// The K largest of the lanes' sorted keys: lane j < K returns the j-th expert and
+// its key without the place.  The lanes' lists lie in shared memory ([lane][V]);
+// a lane holds the head of its list and moves on when it is taken.  *head: the
+// head left at the end, *left how many keys lie before it.
+template <int V>
+SB_DEVINL int take_top(const uint32_t (&key)[V], uint32_t* list, uint32_t* taken, int K, int lane, uint32_t* mine_key,
+                       uint32_t* head_out, int* used) {
+  uint32_t* mylist = list + lane * V;
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int v = 0; v < V; v += 4)
+      *reinterpret_cast<uint4*>(mylist + v) = make_uint4(key[v], key[v + 1], key[v + 2], key[v + 3]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) mylist[v] = key[v];
+  }
+  uint32_t head = key[0];
+  const uint32_t me = 1u << lane;
+  const uint32_t last_id = static_cast<uint32_t>(lane * V) + kPlaceMask<V>;
+  int at = 0;
+  for (int j = 0; j < K; ++j) {
+    const uint32_t h = head & ~kPlaceMask<V>;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, h);
+    const uint32_t who = __ballot_sync(0xffffffffu, h == top);
+    if ((who & (0u - who)) == me) {  // the lowest lane of them
+      *reinterpret_cast<uint2*>(taken + 2 * j) = make_uint2(last_id - (head & kPlaceMask<V>), h);
+      ++at;
+      head = V > 1 && at < V ? mylist[at] : 0;
+    }
+    __syncwarp();
+  }
+  *head_out = head;
+  *used = at;
+  const uint2 t = lane < K ? *reinterpret_cast<const uint2*>(taken + 2 * lane) : make_uint2(0, 0);
+  *mine_key = t.y;
+  return static_cast<int>(t.x);
+}
+
+// The exact form: keys by place in the lane.  Lane j < K returns the j-th expert.
+template <int V>
+SB_DEVINL int take_top_exact(unsigned long long (&key)[V], int K, int lane) {
   int mine = 0;
   for (int j = 0; j < K; ++j) {
-    Key best = key[0];
+    unsigned long long best = key[0];
 #pragma unroll
     for (int v = 1; v < V; ++v) best = key[v] > best ? key[v] : best;
-    const Key top = warp_max_key(best);
+    const unsigned long long top = warp_max_key(best);
     const int winner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
     int at = 0;  // the lowest expert of this lane that has the largest key
 #pragma unroll
@@ -122,31 +193,19 @@ SB_DEVINL int select_top(Key (&key)[V], int K, int lane, Key* mine_key) {
     for (int v = 0; v < V; ++v)
       if (lane == winner && v == at) key[v] = 0;
     const int e = __shfl_sync(0xffffffffu, lane * V + at, winner);
-    if (lane == j) {
-      mine = e;
-      *mine_key = top;
-    }
+    if (lane == j) mine = e;
   }
   return mine;
 }
 
-// Drops the candidates outside the best topk_groups groups; returns whether a
-// group left out came within `tol` of the last one kept.  `ch`: room for the
-// warp's keys of all experts in shared memory, for groups that are not a power
-// of two of whole lanes.
+// Best two keys of each group, in lane g < groups.  k1 / k2: this lane's best
+// two.  Groups of a power of two of whole lanes meet by shuffles; others scan the
+// warp's keys in shared memory.
 template <int V, typename Key>
-SB_DEVINL bool keep_groups(Key (&key)[V], Key* ch, const RouteParams& p, int lane, float tol) {
-  using Val = decltype(key_value(Key(0)));
-  const int per = p.E / p.groups, lanes = per / V;
-  const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
-  Key k1 = 0, k2 = 0;
-  if (whole) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Key lo = key[v] < k1 ? key[v] : k1;
-      k1 = key[v] > k1 ? key[v] : k1;
-      k2 = lo > k2 ? lo : k2;
-    }
+SB_DEVINL void group_best(const Key (&key)[V], Key& k1, Key& k2, Key* ch, const RouteParams& p, int lane,
+                          bool sorted) {
+  if (p.group_shift >= 0) {
+    const int lanes = 1 << p.group_shift;
     for (int o = 1; o < lanes; o <<= 1) {
       const Key o1 = __shfl_xor_sync(0xffffffffu, k1, o), o2 = __shfl_xor_sync(0xffffffffu, k2, o);
       const Key lo = o1 < k1 ? o1 : k1;
@@ -154,53 +213,46 @@ SB_DEVINL bool keep_groups(Key (&key)[V], Key* ch, const RouteParams& p, int lan
       k2 = o2 > k2 ? o2 : k2;
       k2 = lo > k2 ? lo : k2;
     }
-    const int src = lane * lanes < 32 ? lane * lanes : 0;  // from here lane g holds group g
+    const int src = (lane << p.group_shift) & 31;
     k1 = __shfl_sync(0xffffffffu, k1, src);
     k2 = __shfl_sync(0xffffffffu, k2, src);
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (lane * V + v < p.E) ch[lane * V + v] = key[v];
+    for (int v = 0; v < V; ++v) {
+      const int at = lane * V + (sorted ? static_cast<int>(kPlaceMask<V> - (key[v] & kPlaceMask<V>)) : v);
+      if (key[v] != 0 && at < p.E) ch[at] = key[v];
+    }
     __syncwarp();
-    for (int i = 0; lane < p.groups && i < per; ++i) {
-      const Key k = ch[lane * per + i];
+    k1 = k2 = 0;
+    for (int i = 0; lane < p.groups && i < p.per_group; ++i) {
+      const Key k = ch[lane * p.per_group + i];
       if (k > k1) { k2 = k1; k1 = k; } else if (k > k2) k2 = k;
     }
     __syncwarp();
   }
-  Val gs = key_value(k1);
-  if (p.group_top == 2 && per > 1) gs += key_value(k2);
-  const Key gk = lane < p.groups ? order_key(gs) : 0;
-  int rank = 0;  // groups ahead of this lane's
-  for (int g = 0; g < p.groups; ++g) {
-    const Key o = __shfl_sync(0xffffffffu, gk, g);
-    rank += (o > gk || (o == gk && g < lane)) ? 1 : 0;
-  }
-  const bool in = lane < p.groups && rank < p.topk_groups;
-  const uint32_t kept = __ballot_sync(0xffffffffu, in);
-  const int last = __ffs(__ballot_sync(0xffffffffu, lane < p.groups && rank == p.topk_groups - 1)) - 1;
-  const float c = static_cast<float>(__shfl_sync(0xffffffffu, gs, last));
-  const bool near = lane < p.groups && !in && gk >= order_key(static_cast<Val>(c - (tol + fabsf(c) * 0x1p-21f)));
-  if (whole) {
-    const bool mine = (kept >> (lane / lanes & 31)) & 1u;  // lanes past the last expert hold no keys
-#pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = mine ? key[v] : 0;
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = lane * V + v;
-      if (e < p.E && !((kept >> (e / per)) & 1u)) key[v] = 0;
-    }
-  }
-  return __any_sync(0xffffffffu, near);
 }
 
-// The selection from fp64 scores; rare, so it reads the logits again rather
-// than have the caller keep them.
+// Bit mask of the best topk_groups groups, group g's score in lane g; *last is
+// the key of the last one kept, gk afterwards 0 in the kept groups' lanes.
+template <typename Key>
+SB_DEVINL uint32_t best_groups(Key& gk, int topk_groups, int lane, Key* last) {
+  uint32_t kept = 0;
+  for (int j = 0; j < topk_groups; ++j) {
+    *last = warp_max_key(gk);
+    const int g = __ffs(__ballot_sync(0xffffffffu, gk == *last)) - 1;
+    kept |= 1u << g;
+    gk = lane == g ? 0 : gk;
+  }
+  return kept;
+}
+
+// The exact selection: from fp64 scores, or (by_logit) from the logits.  Rare, so
+// it reads the logits again rather than have the caller keep them.
 template <typename T, int V>
-__device__ __noinline__ int select_f64(const T* __restrict__ row, const RouteParams& p, unsigned long long* ch, int lane) {
+__device__ __noinline__ int select_exact(const T* __restrict__ row, const RouteParams& p, bool by_logit,
+                                         unsigned long long* ch, int lane) {
   double m = 0.0, sum = 0.0;
-  if (p.score == SB_SCORE_SOFTMAX) {
+  if (p.score == SB_SCORE_SOFTMAX && !by_logit) {
     float mf = -INFINITY;
     for (int v = 0; v < V; ++v)
       if (lane * V + v < p.E) mf = fmaxf(mf, to_f32<T>(row[lane * V + v]));
@@ -211,7 +263,7 @@ __device__ __noinline__ int select_f64(const T* __restrict__ row, const RoutePar
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  unsigned long long key[V];
+  unsigned long long key[V], k1 = 0, k2 = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = lane * V + v;
@@ -219,24 +271,47 @@ __device__ __noinline__ int select_f64(const T* __restrict__ row, const RoutePar
     if (e < p.E) {
       const float l = to_f32<T>(row[e]), b = p.bias ? p.bias[e] : 0.f;
       const double x = l;
-      const double s = p.score == SB_SCORE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x));
-      key[v] = order_key((l == -INFINITY || b == -INFINITY) ? -INFINITY : s + static_cast<double>(b));
+      double c = x;
+      if (!by_logit) {
+        const double s = p.score == SB_SCORE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x));
+        c = (l == -INFINITY || b == -INFINITY) ? -INFINITY : s + static_cast<double>(b);
+      }
+      key[v] = order_key(c);
+    }
+    const unsigned long long lo = key[v] < k1 ? key[v] : k1;
+    k1 = key[v] > k1 ? key[v] : k1;
+    k2 = lo > k2 ? lo : k2;
+  }
+  if (p.topk_groups < p.groups) {
+    group_best<V>(key, k1, k2, ch, p, lane, false);
+    double gs = key_value(k1);
+    if (p.group_top == 2 && p.per_group > 1) gs += key_value(k2);
+    unsigned long long gk = lane < p.groups ? order_key(gs) : 0, last;
+    const uint32_t kept = best_groups(gk, p.topk_groups, lane, &last);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = lane * V + v;
+      if (e < p.E && !((kept >> (e / p.per_group)) & 1u)) key[v] = 0;
     }
   }
-  if (p.topk_groups < p.groups) keep_groups<V>(key, ch, p, lane, 0.f);
-  unsigned long long unused;
-  return select_top<V>(key, p.K, lane, &unused);
+  return take_top_exact<V>(key, p.K, lane);
 }
 
+// Shared memory per warp: the lanes' lists and the K experts taken, or (exact
+// selection) fp64 keys of all experts.
+template <int V>
+constexpr int kRouteSmem = 32 * V * 8 + kRouteMaxK * 8;
+
 template <typename T, int V, bool kVec>
-__global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict__ logits, const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict__ logits,
+                                                            const __grid_constant__ RouteParams p) {
   extern __shared__ __align__(16) uint8_t route_smem[];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp;
   if (t >= p.n) return;
-  unsigned long long* ch = reinterpret_cast<unsigned long long*>(route_smem) + static_cast<size_t>(warp) * p.E;
+  unsigned long long* ch = reinterpret_cast<unsigned long long*>(route_smem + warp * kRouteSmem<V>);
   const T* row = logits + t * p.ld;
   const bool softmax = p.score == SB_SCORE_SOFTMAX;
   const bool grouped = p.topk_groups < p.groups;
@@ -244,66 +319,105 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
   const bool by_logit = !p.bias && !(grouped && p.group_top == 2);
   float l[V];
   load_logits<T, V, kVec>(row, p.E, lane, l);
-  float m = -INFINITY, sum = 0.f, inv = 0.f, s[V];
+  float m = -INFINITY, sum = 0.f, inv = 0.f, c[V];
   if (softmax) {
 #pragma unroll
     for (int v = 0; v < V; ++v) m = fmaxf(m, l[v]);
     m = warp_max(m);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      s[v] = l[v] == -INFINITY ? 0.f : expf(l[v] - m);
-      sum += s[v];
+      c[v] = l[v] == -INFINITY ? 0.f : expf(l[v] - m);
+      sum += c[v];
     }
     sum = warp_sum(sum);
     inv = sum == 0.f ? 0.f : 1.f / sum;
   }
+  if (by_logit) {
+    const float nan = 0.f * sum;  // a NaN anywhere in a softmax row makes every score of the row NaN
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = l[v] + nan;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      // the fast sigmoid is off by (1.5 |x| + 4) s (1 - s) 2^-23, below 2^-21
+      c[v] = softmax ? c[v] * inv : rcp_approx(1.f + __expf(-l[v]));
+    if (p.bias) {
+      float b[V];
+      load_logits<float, V, kVec>(p.bias, p.E, lane, b);
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] += b[v];
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) c[v] = l[v] == -INFINITY ? -INFINITY : c[v];
   uint32_t key[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane * V + v;
-    float c;
-    if (by_logit) {
-      c = l[v] + 0.f * sum;  // a NaN anywhere in a softmax row makes every score of the row NaN
-    } else {
-      const float b = e < p.E && p.bias ? p.bias[e] : 0.f;
-      // the fast sigmoid: (1.5 |x| + 4) s (1 - s) 2^-23 off, below 2^-21
-      const float sc = softmax ? s[v] * inv : __fdividef(1.f, 1.f + __expf(-l[v]));
-      c = (l[v] == -INFINITY || b == -INFINITY) ? -INFINITY : sc + b;
-    }
-    key[v] = e < p.E ? order_key(c) : 0;
-  }
+  for (int v = 0; v < V; ++v)
+    key[v] = lane * V + v < p.E ? (order_key(c[v]) & ~kPlaceMask<V>) | (kPlaceMask<V> - v) : 0;
+  sort_descending<V>(key);
   // fp32 error of a score: exp of a rounded difference (|x| e^-|x| 2^-24 <=
-  // 0.37 2^-24), 2 ulp of expf, the sum and the division, all below 2^-20 in
-  // all; two of them may differ by 2^-19.
-  constexpr float kTol = 0x1p-19f;
+  // 0.37 2^-24), 2 ulp of expf, the sum and the division, all below 2^-20 in all;
+  // two may differ by 2^-19.  Rounding of a choice: 2^-24 of it, and V of its
+  // last places for the expert's place.
+  constexpr float kTol = 0x1p-19f, kRel = (V + 1) * 0x1p-22f;
+  // by_logit: the keys order exactly, but for the bits the place took (a bf16
+  // logit has none there)
+  const bool exact = by_logit && sizeof(T) == 2;
   bool close = false;
-  if (grouped) close = keep_groups<V>(key, reinterpret_cast<uint32_t*>(ch), p, lane, 2.f * kTol);
-  uint32_t mine_key = 0;
-  int mine = select_top<V>(key, p.K, lane, &mine_key);
+  if (grouped) {
+    uint32_t k1 = key[0], k2 = V > 1 ? key[V > 1 ? 1 : 0] : 0;
+    group_best<V>(key, k1, k2, reinterpret_cast<uint32_t*>(ch), p, lane, true);
+    float gs = place_key_value(k1 & ~kPlaceMask<V>);
+    if (p.group_top == 2 && p.per_group > 1) gs += place_key_value(k2 & ~kPlaceMask<V>);
+    uint32_t gk = lane < p.groups ? order_key(gs) : 0, last;
+    const uint32_t kept = best_groups(gk, p.topk_groups, lane, &last);
+    const float lc = key_value(last);
+    const uint32_t limit = by_logit ? last : order_key(lc - (2.f * kTol + 2.f * fabsf(lc) * kRel));
+    close = !exact && gk != 0 && gk >= limit;  // a group left out so close to the last one kept
+    if (p.group_shift >= 0) {
+      if (!((kept >> (lane >> p.group_shift)) & 1u)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = 0;
+      }
+    } else {
+      for (int v = 0; v < V; ++v) {
+        const int e = lane * V + static_cast<int>(kPlaceMask<V> - (key[v] & kPlaceMask<V>));
+        if (!((kept >> ((e / p.per_group) & 31)) & 1u)) key[v] = 0;
+      }
+      sort_descending<V>(key);  // the dropped ones to the end
+    }
+  }
+  uint32_t mine_key, head;
+  int used;
+  uint32_t* list = reinterpret_cast<uint32_t*>(ch);
+  int mine = take_top<V>(key, list, list + 32 * V, p.K, lane, &mine_key, &head, &used);
   float ls = lane < p.K ? to_f32<T>(row[mine]) : -INFINITY;
   float bs = lane < p.K && p.bias ? p.bias[mine] : 0.f;
-  if (!by_logit) {
+  if (!exact) {
     // Did a decision hang on a gap that fp32 does not resolve?  Between one taken
     // expert and the next, or between the last taken and one left out, unless
     // the two are exactly equal (same logit, same bias).  (If such a gap lies
     // further up, the experts between are exactly equal to its upper end.)
-    const float c = key_value(mine_key);
-    const float pc = __shfl_up_sync(0xffffffffu, c, 1), pl = __shfl_up_sync(0xffffffffu, ls, 1),
-                pb = __shfl_up_sync(0xffffffffu, bs, 1);
-    if (lane > 0 && lane < p.K && pc - c <= kTol + fabsf(pc) * 0x1p-22f && (pl != ls || pb != bs)) close = true;
-    const float lc = __shfl_sync(0xffffffffu, c, p.K - 1);
-    const uint32_t limit = order_key(lc - (kTol + fabsf(lc) * 0x1p-22f));
-    bool near = false;
-#pragma unroll
-    for (int v = 0; v < V; ++v) near |= key[v] >= limit;
-    if (__any_sync(0xffffffffu, near)) {
+    const uint32_t pk = __shfl_up_sync(0xffffffffu, mine_key, 1);
+    const float pl = __shfl_up_sync(0xffffffffu, ls, 1), pb = __shfl_up_sync(0xffffffffu, bs, 1);
+    const float cm = place_key_value(mine_key), pc = place_key_value(pk);
+    const bool tight = by_logit ? pk == mine_key : pc - cm <= kTol + fabsf(pc) * kRel;
+    close |= lane > 0 && lane < p.K && tight && (pl != ls || pb != bs);
+    const uint32_t lk = __shfl_sync(0xffffffffu, mine_key, p.K - 1);
+    const float lc = place_key_value(lk);
+    const uint32_t limit = by_logit ? lk : order_key(lc - (kTol + fabsf(lc) * kRel));
+    if (__any_sync(0xffffffffu, head >= limit)) {
       const float ll = __shfl_sync(0xffffffffu, ls, p.K - 1), lb = __shfl_sync(0xffffffffu, bs, p.K - 1);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (key[v] >= limit && key[v] != 0 && (l[v] != ll || (p.bias ? p.bias[lane * V + v] : 0.f) != lb)) close = true;
+      for (int v = used; v < V; ++v) {
+        const uint32_t k = list[lane * V + v];
+        if (k < limit || k == 0) break;
+        const int e = lane * V + static_cast<int>(kPlaceMask<V> - (k & kPlaceMask<V>));
+        close |= to_f32<T>(row[e]) != ll || (p.bias ? p.bias[e] : 0.f) != lb;
+      }
+      __syncwarp();
     }
     if (__any_sync(0xffffffffu, close)) {
-      mine = select_f64<T, V>(row, p, ch, lane);
+      mine = select_exact<T, V>(row, p, by_logit && sum == sum, ch, lane);
       ls = lane < p.K ? to_f32<T>(row[mine]) : -INFINITY;
       bs = lane < p.K && p.bias ? p.bias[mine] : 0.f;
     }
@@ -429,13 +543,17 @@ static bool route_vec(const void* base, int64_t ld, int E) {
 }
 
 template <typename T, int V>
-static int launch_route(const void* logits, const RouteParams& p, cudaStream_t st) {
+static int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
   const int warps = route_warps(p.E);
-  // keys of the group scan: 4 bytes an expert, 8 in the fp64 selection
-  const size_t smem = p.topk_groups < p.groups ? static_cast<size_t>(warps) * p.E * 8 : 0;  // at most 32 KB
+  const size_t smem = static_cast<size_t>(warps) * kRouteSmem<V>;  // at most 33 KB
+  const int lanes = p.per_group / V;
+  if (lanes * V == p.per_group && (lanes & (lanes - 1)) == 0) {
+    p.group_shift = 0;
+    while ((1 << p.group_shift) < lanes) ++p.group_shift;
+  }
   const dim3 grid((p.n + warps - 1) / warps), block(warps * 32);
   if constexpr (V >= 4) {
-    if (route_vec<T, V>(logits, p.ld, p.E))
+    if (route_vec<T, V>(logits, p.ld, p.E) && (!p.bias || reinterpret_cast<uintptr_t>(p.bias) % 16 == 0))
       return launch(route_experts_kernel<T, V, true>, grid, block, smem, st, static_cast<const T*>(logits), p);
   }
   return launch(route_experts_kernel<T, V, false>, grid, block, smem, st, static_cast<const T*>(logits), p);
@@ -489,7 +607,7 @@ extern "C" SB_API int sb_route_experts(const void* logits, int dtype, int64_t ld
   if (n_tokens == 0) return SB_OK;
   if (!logits || !top_idx || !top_w) return SB_ERR_ARG;
   RouteParams p = {ld, n_tokens, num_experts, top_k, score, bias, num_groups, topk_groups, group_top, renormalize,
-                   scale, top_idx, top_w};
+                   scale, top_idx, top_w, num_experts / num_groups, -1};
   SB_ROUTE_DISPATCH(launch_route, logits, p, static_cast<cudaStream_t>(stream));
 }
 
@@ -502,6 +620,6 @@ extern "C" SB_API int sb_route_experts_backward(const void* logits, int dtype, i
   if (n_tokens == 0) return SB_OK;
   if (!logits || !top_idx || !grad_w || !grad_logits) return SB_ERR_ARG;
   RouteParams p = {ld, n_tokens, num_experts, top_k, score, bias, 1, 1, 1, renormalize, scale,
-                   const_cast<int32_t*>(top_idx), nullptr};
+                   const_cast<int32_t*>(top_idx), nullptr, num_experts, -1};
   SB_ROUTE_DISPATCH(launch_route_backward, logits, p, grad_w, grad_logits, ld_grad, static_cast<cudaStream_t>(stream));
 }
