@@ -23,16 +23,19 @@
 // rows of a and half of the weight rows, which halves the weight traffic into
 // shared memory, the limit of the one-CTA tile.
 //
-// Warps: 0-15 epilogue (TMEM lane quarter w % 4, columns part w / 4), 16 TMA, 17
-// MMA (+TMEM).  Every wait is bounded (sb_common.cuh); loads use no multicast.
+// Scales come through shared memory from a warp of their own: a block's scales
+// are loaded two blocks ahead, multiplied, and written to the slot of the
+// accumulator they belong to once that accumulator was read.  The same arrival
+// tells the MMA thread that the accumulator is free, so it waits for one barrier
+// per block, full (operands landed, accumulator free), and signals one, done.
+//
+// Warps: 0-7 epilogue (TMEM lane quarter w % 4, columns part w / 4), 8 TMA, 9
+// MMA (+TMEM), 10 scales.  Every wait is bounded (sb_common.cuh); loads use no
+// multicast.
 #include "sb_fp8.cuh"
 #include "sb_gemm_common.cuh"
 #include "sb_internal.h"
 
-#ifndef F8_PARTS
-#define F8_PARTS 2
-#define F8_CHUNK 32
-#endif
 namespace sb {
 
 constexpr int kF8MaxG = 1024;
@@ -49,15 +52,14 @@ struct F8Cfg {
   static constexpr int kStages = 4;
   static constexpr int kAccCols = 2 * kHalf;
   static constexpr int kTmemCols = 2 * kAccCols;
-  static constexpr int kParts = F8_PARTS;                     // epilogue warps per TMEM lane quarter
+  static constexpr int kParts = 2;                     // epilogue warps per TMEM lane quarter
   static constexpr int kCols = kHalf / kParts;         // columns of each half per epilogue thread
   static constexpr int kEpiWarps = 4 * kParts;
-  static constexpr int kChunk = F8_CHUNK;              // columns per TMEM load
+  static constexpr int kChunk = 32;                    // columns per TMEM load
   static constexpr int kThreads = (kEpiWarps + 4) * 32;  // whole warpgroups: registers move between them
   // Registers per thread at launch (65536 / kThreads, in steps of 8) and after
   // the split.
-  static constexpr int kRegsLaunch = kParts == 2 ? 168 : 96;
-  static constexpr int kRegsEpi = kParts == 2 ? 224 : 104, kRegsLoad = kParts == 2 ? 56 : 64;
+  static constexpr int kRegsLaunch = 168, kRegsEpi = 224, kRegsLoad = 56;
   static_assert(kEpiWarps * 32 * kRegsEpi + 128 * kRegsLoad <= kThreads * kRegsLaunch, "the split must fit the launch's registers");
   static constexpr int kSmallRows = 32;                // rows of the box that short tiles load
   static constexpr int kOffA = 0;
@@ -66,21 +68,65 @@ struct F8Cfg {
   static constexpr int kBoxBytes = 32 * 128;
   static constexpr int kOffOut = kOffB + kStages * kBBytes;
   static constexpr int kOffBar = kOffOut + (kPair ? kEpiWarps * 2 * kBoxBytes : 0);
-  static constexpr int kOffMisc = kOffBar + (2 * kStages + 4) * 8;
-  static constexpr int kOffMax = kOffMisc + 64;                            // uint32 [2 blocks][kParts][128 rows]
-  static constexpr int kOffBScale = kOffMax + 2 * kParts * kBM * 4;        // float [warps][2][kCols]
-  static constexpr int kOffPrefix = kOffBScale + kEpiWarps * 2 * kCols * 4;  // int [kF8MaxG + 1]
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + 2) * 8;
+  static constexpr int kOffMax = (kOffMisc + 64 + 15) / 16 * 16;                            // uint32 [2 blocks][kParts][128 rows]
+  static constexpr int kOffBias = kOffMax + 2 * kParts * kBM * 4;          // float [warps][2][kCols]
+  static constexpr int kOffScale = kOffBias + kEpiWarps * 2 * kCols * 4;   // float [2 accumulators][kScaleFloats]
+  static constexpr int kScaleFloats = kBM + 2 * kHalf;  // [2][128 rows] products, or [128] a and [256] b (kBRows)
+  static constexpr int kOffPrefix = kOffScale + 2 * kScaleFloats * 4;      // int [kF8MaxG + 1]
   static constexpr int kOffOffsets = kOffPrefix + (kF8MaxG + 1) * 4;
   static constexpr int kSmemBytes = kOffOffsets + (kF8MaxG + 1) * 4 + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(kTmemCols == 512, "two accumulators of 256 columns");
-  static_assert(kOffBScale % 16 == 0, "float2 reads");
+  static_assert(kOffBias % 16 == 0 && kOffScale % 16 == 0, "16-byte reads");
 };
 
 // Instruction descriptor: e4m3 x e4m3 -> fp32, both K-major, M x N tile.
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
+
+// Operand descriptors (K-major, 128-byte swizzle; smem_desc_k_sw128) in halves:
+// the upper one is constant, the lower one counts 16-byte units, so a stage or a
+// step of 32 elements is one addition.  The MMA loop is one thread's chain of
+// dependent instructions, and at four short MMAs a round its length shows: with
+// descriptors built from addresses, stage numbers from divisions and a barrier of
+// its own for the accumulators, a round took 460-500 ns where its MMAs take 260.
+constexpr uint32_t kF8DescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+SB_DEVINL uint32_t f8_desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
+SB_DEVINL uint64_t f8_desc(uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "n"(kF8DescHi));
+  return d;
+}
+// One lane of a converged warp, which runs the TMA or the MMA loop.  Elected rather
+// than `lane == 0`, so that the compiler knows there is one thread: the operands of
+// tcgen05.mma and of the TMA copies are uniform registers, and filling them from a
+// divergent warp made the four MMAs of a block take 400 clocks to issue (157 so).
+SB_DEVINL bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+SB_DEVINL const float* sa_ptr_at(const float* p, int j, int64_t row, int kk, int64_t block) {
+  return p + 32 * j * row + kk * block;
+}
+// A position in a ring of kN slots and the parity of the current round.
+template <int kN>
+struct Ring {
+  int slot = 0;
+  uint32_t parity = 0;
+  SB_DEVINL void next() {
+    if (++slot == kN) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
 
 template <bool kPair>
 SB_DEVINL void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -129,10 +175,10 @@ SB_DEVINL void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[kN / 2]) {
 #pragma unroll
   for (int i = 0; i < kN / 2; ++i) asm("mov.b64 %0, {%1, %2};" : "=l"(v[i]) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
 }
-// Arrive on the leader's accumulator barrier.  What it hands over is TMEM, ordered
-// by the tcgen05 fences on both sides, so the default CTA-scope release does: a
-// cluster-scope one waits for every outstanding access of the thread, once per
-// block of k (measured on 16384 x 4096 x 8192: 1190 us with it).
+// Arrive on a barrier of the pair's leader.  What it hands over is an accumulator,
+// ordered by the tcgen05 fences on both sides, so the default CTA-scope release
+// does: a cluster-scope one waits for every outstanding access of the thread,
+// once per block of k (16384 x 4096 x 8192: 1190 us with it, 685 us without).
 SB_DEVINL void mbar_arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -220,18 +266,20 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   constexpr bool kGate = EPI == SB_EPI_SWIGLU;
   constexpr bool kQuant = EPI != SB_EPI_LINEAR;
   constexpr int kTileCols = kGate ? C::kHalf : 2 * C::kHalf;
-  constexpr int kTmaWarp = C::kEpiWarps, kMmaWarp = C::kEpiWarps + 1;
+  constexpr int kTmaWarp = C::kEpiWarps, kMmaWarp = C::kEpiWarps + 1, kScaleWarp = C::kEpiWarps + 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // a pair uses the leader's
-  uint64_t* empty = full + S;
-  uint64_t* acc_full = empty + S;      // [2]
-  uint64_t* acc_empty = acc_full + 2;  // [2], a pair uses the leader's
+  // A block's MMAs are done: its stage is free and its accumulator is complete.
+  // (S >= 2: the MMAs of the stage's next use wait for acc_empty of this one.)
+  uint64_t* done = full + S;
+  uint64_t* acc_empty = done + S;  // [2]: this CTA's epilogue has read accumulator and scales
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
   const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
   const int first = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int stride = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
@@ -240,13 +288,10 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   const int nk = (p.k + C::kBK - 1) / C::kBK;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&full[s], 1 + (kPair ? 2 : 1));  // the copies, and each CTA's scale warp
+      mbar_init(&done[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], C::kEpiWarps * (kPair ? 2 : 1));
-    }
+    for (int b = 0; b < 2; ++b) mbar_init(&acc_empty[b], C::kEpiWarps);
     fence_barrier_init();
   }
   if (warp == kTmaWarp && lane == 0) {
@@ -307,78 +352,139 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLoad));
     if (warp == kTmaWarp) {
     // ---------------------------------------------------------------- TMA
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int t = first; t < total && ok; t += stride) {
-        const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
-        const bool second = kGate || w.n0 + C::kHalf < p.n;  // the tile's second 128 weight rows exist
-        const int brow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
-        auto a_bytes = [&](int rows) {  // a CTA without rows loads none: its lanes are never read
-          return static_cast<uint32_t>(rows <= 0 ? 0 : (rows <= C::kSmallRows ? C::kSmallRows * C::kBK : C::kABytes));
-        };
-        const uint32_t tx = kPair ? a_bytes(w.rows) + a_bytes(w.peer) + 2 * C::kHalfBytes
-                                  : a_bytes(w.rows) + C::kHalfBytes * (second ? 2 : 1);
-        const CUtensorMap* map_a = w.rows <= C::kSmallRows ? &tmAs : &tmA;
-        for (int kk = 0; kk < nk; ++kk, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
-          const int k0 = kk * C::kBK;
-          uint8_t* adst = smem + C::kOffA + s * C::kABytes;
-          uint8_t* bdst = smem + C::kOffB + s * C::kBBytes;
-          if constexpr (kPair) {
-            // both CTAs' bytes count on the leader's barrier.  The MMA takes the
-            // first half of its N columns from CTA 0, the second from CTA 1.
-            if (rank == 0) mbar_expect_tx(&full[s], tx);
-            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-            tma_load_2d_pair(bdst, kGate && rank == 0 ? &tmG : &tmB, bar, k0,
-                             kGate || rank == 0 ? brow : brow + (second ? C::kHalf : C::kHalf / 2));
-            if (w.rows > 0) tma_load_2d_pair(adst, map_a, bar, k0, w.row0);
-          } else {
-            mbar_expect_tx(&full[s], tx);
-            tma_load_2d(bdst, kGate ? &tmG : &tmB, &full[s], k0, brow);
-            if (second) tma_load_2d(bdst + C::kHalfBytes, &tmB, &full[s], k0, kGate ? brow : brow + C::kHalf);
-            tma_load_2d(adst, map_a, &full[s], k0, w.row0);
+      if (elect_one()) {
+        Ring<S> st;
+        int issued = 0;
+        bool ok = true;
+        for (int t = first; t < total && ok; t += stride) {
+          const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
+          const bool second = kGate || w.n0 + C::kHalf < p.n;  // the tile's second 128 weight rows exist
+          const int brow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
+          auto a_bytes = [&](int rows) {  // a CTA without rows loads none: its lanes are never read
+            return static_cast<uint32_t>(rows <= 0 ? 0 : (rows <= C::kSmallRows ? C::kSmallRows * C::kBK : C::kABytes));
+          };
+          const uint32_t tx = kPair ? a_bytes(w.rows) + a_bytes(w.peer) + 2 * C::kHalfBytes
+                                    : a_bytes(w.rows) + C::kHalfBytes * (second ? 2 : 1);
+          const CUtensorMap* map_a = w.rows <= C::kSmallRows ? &tmAs : &tmA;
+          for (int kk = 0; kk < nk; ++kk, st.next()) {
+            uint64_t* const bar = &full[st.slot];
+            if (!mbar_wait(&done[st.slot], st.parity ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
+            if (issued < S) ++issued;
+            const int k0 = kk * C::kBK;
+            uint8_t* adst = smem + C::kOffA + st.slot * C::kABytes;
+            uint8_t* bdst = smem + C::kOffB + st.slot * C::kBBytes;
+            if constexpr (kPair) {
+              // both CTAs' bytes count on the leader's barrier.  The MMA takes the
+              // first half of its N columns from CTA 0, the second from CTA 1.
+              if (rank == 0) mbar_expect_tx(bar, tx);
+              const uint32_t lead = mapa_shared(smem_u32(bar), 0);
+              tma_load_2d_pair(bdst, kGate && rank == 0 ? &tmG : &tmB, lead, k0,
+                               kGate || rank == 0 ? brow : brow + (second ? C::kHalf : C::kHalf / 2));
+              if (w.rows > 0) tma_load_2d_pair(adst, map_a, lead, k0, w.row0);
+            } else {
+              mbar_expect_tx(bar, tx);
+              tma_load_2d(bdst, kGate ? &tmG : &tmB, bar, k0, brow);
+              if (second) tma_load_2d(bdst + C::kHalfBytes, &tmB, bar, k0, kGate ? brow : brow + C::kHalf);
+              tma_load_2d(adst, map_a, bar, k0, w.row0);
+            }
+          }
+        }
+        // every stage done with: all copies landed and all commit arrivals in
+        for (int i = 0; i < issued; ++i, st.next()) {
+          const int slot = (st.slot + S - issued) % S;
+          if (!mbar_wait(&done[slot], (st.slot >= issued ? st.parity : st.parity ^ 1), p.status, SB_DEVERR_DRAIN)) break;
+        }
+      }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA (a pair's leader)
+      if (rank == 0 && elect_one()) {
+        Ring<S> st;
+        Ring<2> acc;
+        const uint32_t a_lo = f8_desc_lo(smem_u32(smem + C::kOffA)), b_lo = f8_desc_lo(smem_u32(smem + C::kOffB));
+        bool ok = true;
+        for (int t = first; t < total && ok; t += stride) {
+          const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
+          const bool second = kGate || w.n0 + C::kHalf < p.n;
+          const uint32_t idesc = idesc_e4m3_f32(C::kItemRows, second ? 2 * C::kHalf : C::kHalf);
+          for (int kk = 0; kk < nk; ++kk, st.next(), acc.next()) {
+            if (!mbar_wait(&full[st.slot], st.parity, p.status, SB_DEVERR_TMA_WAIT)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t al = a_lo + st.slot * (C::kABytes >> 4), bl = b_lo + st.slot * (C::kBBytes >> 4);
+#pragma unroll
+            for (int q = 0; q < C::kBK / 32; ++q)
+              tc_mma_f8<kPair>(tmem + acc.slot * C::kAccCols, f8_desc(al + 2 * q), f8_desc(bl + 2 * q), idesc, q > 0);
+            if constexpr (kPair) tc_commit_pair(&done[st.slot]);
+            else tc_commit(&done[st.slot]);
           }
         }
       }
-      // every stage released: all copies landed and all commit arrivals done
-      for (int i = it - S > 0 ? it - S : 0; i < it; ++i)
-        if (!mbar_wait(&empty[i % S], (i / S) & 1, p.status, SB_DEVERR_DRAIN)) break;
-    }
-    __syncwarp();
-    } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- MMA (a pair's leader)
-    if (lane == 0 && rank == 0) {
-      int it = 0;
+      __syncwarp();
+    } else if (warp == kScaleWarp) {
+      // ---------------------------------------------------------------- scales
+      Ring<S> st;
+      Ring<2> acc;
       bool ok = true;
       for (int t = first; t < total && ok; t += stride) {
         const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
         const bool second = kGate || w.n0 + C::kHalf < p.n;
-        const uint32_t idesc = idesc_e4m3_f32(C::kItemRows, second ? 2 * C::kHalf : C::kHalf);
-        for (int kk = 0; kk < nk; ++kk, ++it) {
-          const int s = it % S, buf = it & 1;
-          ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, p.status, SB_DEVERR_EPI_WAIT) &&
-               mbar_wait(&full[s], (it / S) & 1, p.status, SB_DEVERR_TMA_WAIT);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t a_base = smem_u32(smem + C::kOffA + s * C::kABytes);
-          const uint32_t b_base = smem_u32(smem + C::kOffB + s * C::kBBytes);
+        const float* sa_ptr = p.a_scale + static_cast<int64_t>(w.row0 + lane) * p.a_scale_row;
+        const float* sb0 = (kGate ? p.b_gate_scale : p.b_scale) + w.g * p.b_scale_group;
+        const float* sb1 = p.b_scale + w.g * p.b_scale_group;
+        if (!kBRows) {
+          sb0 += (w.n0 / 128) * p.b_scale_row;
+          sb1 += (w.n0 / 128 + (kGate ? 0 : 1)) * p.b_scale_row;
+        } else {
+          sb1 += static_cast<int64_t>(w.n0 + lane) * p.b_scale_row;
+        }
+        constexpr int kAhead = 2, kB = kBRows ? 8 : 2;
+        float sa[kAhead][4], sb[kAhead][kB];
+        auto load = [&](int kk, int i) {
+          if (kk >= nk) return;
 #pragma unroll
-          for (int q = 0; q < C::kBK / 32; ++q)
-            tc_mma_f8<kPair>(tmem + buf * C::kAccCols, smem_desc_k_sw128(a_base + q * 32),
-                             smem_desc_k_sw128(b_base + q * 32), idesc, q > 0);
-          if constexpr (kPair) {
-            tc_commit_pair(&empty[s]);
-            tc_commit_pair(&acc_full[buf]);
+          for (int j = 0; j < 4; ++j) {
+            sa[i][j] = lane + 32 * j < w.rows ? *sa_ptr_at(sa_ptr, j, p.a_scale_row, kk, p.a_scale_block) : 0.f;
+          }
+          if (kBRows) {
+#pragma unroll
+            for (int j = 0; j < kB; ++j)
+              sb[i][j] = w.n0 + lane + 32 * j < p.n ? *sa_ptr_at(sb1, j, p.b_scale_row, kk, p.b_scale_block) : 0.f;
           } else {
-            tc_commit(&empty[s]);
-            tc_commit(&acc_full[buf]);
+            sb[i][0] = sb0[kk * p.b_scale_block];
+            sb[i][1] = second ? sb1[kk * p.b_scale_block] : 0.f;
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load(i, i);
+        for (int kk0 = 0; kk0 < nk && ok; kk0 += kAhead) {
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (kk0 + i >= nk) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[acc.slot], acc.parity ^ 1, p.status, SB_DEVERR_EPI_WAIT))) {
+              ok = false;
+              break;
+            }
+            float* f = reinterpret_cast<float*>(smem + C::kOffScale) + acc.slot * C::kScaleFloats;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f[lane + 32 * j] = kBRows ? sa[i][j] : sa[i][j] * sb[i][0];
+              if (!kBRows) f[C::kBM + lane + 32 * j] = sa[i][j] * sb[i][1];
+            }
+            if (kBRows) {
+#pragma unroll
+              for (int j = 0; j < kB; ++j) f[C::kBM + lane + 32 * j] = sb[i][j];
+            }
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kPair) mbar_arrive_leader(mapa_shared(smem_u32(&full[st.slot]), 0));
+              else mbar_arrive(&full[st.slot]);
+            }
+            st.next();
+            acc.next();
+            load(kk0 + i + kAhead, i);
           }
         }
       }
-    }
-    __syncwarp();
     }
   } else {
     // ---------------------------------------------------------------- epilogue
@@ -387,9 +493,9 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const int quarter = warp & 3, part = warp >> 2;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * NC;
     uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
-    float* s_bs = reinterpret_cast<float*>(smem + C::kOffBScale) + warp * 2 * NC;
-    const uint32_t acc_empty_addr = kPair ? mapa_shared(smem_u32(acc_empty), 0) : 0;
-    int it = 0;
+    float* s_bs = reinterpret_cast<float*>(smem + C::kOffBias) + warp * 2 * NC;
+    Ring<S> st;
+    int buf = 0;
     bool ok = true;
     for (int t = first; t < total && ok; t += stride) {
       const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
@@ -398,14 +504,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       const bool warp_live = quarter * 32 < w.rows;
       const bool second = kGate || w.n0 + C::kHalf < p.n;
       const int64_t row = w.row0 + r;
-      const float* sa_ptr = p.a_scale + row * p.a_scale_row;
-      const float* sb0 = (kGate ? p.b_gate_scale : p.b_scale) + w.g * p.b_scale_group;
-      const float* sb1 = p.b_scale + w.g * p.b_scale_group;
-      if (!kBRows) {
-        sb0 += (w.n0 / 128) * p.b_scale_row;
-        sb1 += (w.n0 / 128 + (kGate ? 0 : 1)) * p.b_scale_row;
-      }
-      // kBRows: a lane stages the scales of NC / 16 of the warp's 2 NC columns
+      // this lane's share of the warp's 2 NC bias values
       constexpr int NB = NC / 16;
       const int bcol = w.n0 + (lane >> 4) * C::kHalf + part * NC + (lane & 15) * NB;
       uint64_t sum[2][NC / 2];
@@ -413,40 +512,24 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
-      // scales of block kk are loaded one block ahead: their latency is longer
-      // than a block's MMAs
-      float sa = live ? sa_ptr[0] : 0.f;
-      float p0 = 0.f, p1 = 0.f, pb[NB] = {};
-      auto load_b_scales = [&](int kk) {
-        if (kBRows) {
+      // 0 without a bias, and past n; staged below once the sums are complete
+      float pbias[NB];
+      {
+        const float* bias = kGate && lane < 16 ? p.bias_gate : p.bias;
+        const int c0 = kGate ? w.n0 + part * NC + (lane & 15) * NB : bcol;
 #pragma unroll
-          for (int j = 0; j < NB; ++j)
-            if (bcol + j < p.n) pb[j] = sb1[(bcol + j) * p.b_scale_row + kk * p.b_scale_block];
-        } else {
-          p0 = sb0[kk * p.b_scale_block];
-          if (second) p1 = sb1[kk * p.b_scale_block];
-        }
-      };
-      load_b_scales(0);
-      for (int kk = 0; kk < nk; ++kk, ++it) {
-        const int buf = it & 1;
-        const uint64_t s0 = pair_of(kBRows ? sa : sa * p0), s1 = pair_of(kBRows ? sa : sa * p1);
-        if (kBRows) {
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < NB; ++j) s_bs[lane * NB + j] = pb[j];
-          __syncwarp();
-        }
-        if (kk + 1 < nk) {
-          if (live) sa = sa_ptr[(kk + 1) * p.a_scale_block];
-          load_b_scales(kk + 1);
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
+        for (int j = 0; j < NB; ++j)
+          pbias[j] = bias && c0 + j < p.n ? bias[w.g * p.bias_group + c0 + j] : 0.f;
+      }
+      for (int kk = 0; kk < nk; ++kk, st.next(), buf ^= 1) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&done[st.slot], st.parity, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t t0 = lane_addr + buf * C::kAccCols;
+        const float* f = reinterpret_cast<const float*>(smem + C::kOffScale) + buf * C::kScaleFloats;
+        const uint64_t s0 = pair_of(f[r]), s1 = kBRows ? s0 : pair_of(f[C::kBM + r]);
         constexpr int CH = C::kChunk;
         constexpr int kLoads = 2 * NC / CH;
         uint64_t v[CH / 2];
@@ -454,10 +537,16 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         auto add = [&](int j) {
           const int h = j * CH / NC, c = j * CH % NC;
 #pragma unroll
-          for (int i = 0; i < CH / 2; ++i)
-            fma_pair(sum[h][c / 2 + i],
-                     kBRows ? mul_pair(v[i], *reinterpret_cast<const uint64_t*>(s_bs + h * NC + c + 2 * i)) : v[i],
-                     h ? s1 : s0);
+          for (int i = 0; i < CH / 2; i += 2) {
+            if (kBRows) {
+              const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(f + C::kBM + h * C::kHalf + part * NC + c + 2 * i);
+              fma_pair(sum[h][c / 2 + i], mul_pair(v[i], b.x), s0);
+              fma_pair(sum[h][c / 2 + i + 1], mul_pair(v[i + 1], b.y), s0);
+            } else {
+              fma_pair(sum[h][c / 2 + i], v[i], h ? s1 : s0);
+              fma_pair(sum[h][c / 2 + i + 1], v[i + 1], h ? s1 : s0);
+            }
+          }
         };
         if (warp_live) {
 #pragma unroll
@@ -467,15 +556,17 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               add(j);
             }
           if (second) load(kLoads - 1);
+          if (kBRows && second) add(kLoads - 1);  // reads the slot's scales
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (kPair) mbar_arrive_leader(acc_empty_addr + 8u * buf);
-          else mbar_arrive(&acc_empty[buf]);
-        }
-        if (warp_live && second) add(kLoads - 1);
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        if (!kBRows && warp_live && second) add(kLoads - 1);
       }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < NB; ++j) s_bs[lane * NB + j] = pbias[j];
+      __syncwarp();
       float acc[2][NC];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -500,12 +591,16 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           const int valid = p.n - c0;
           if (valid <= 0) continue;
           if (p.bias) {
-            const float* bias = p.bias + w.g * p.bias_group + c0;
 #pragma unroll
-            for (int i = 0; i < NC; ++i) acc[h][i] += i < valid ? bias[i] : 0.f;
+            for (int i = 0; i < NC; i += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(s_bs + h * NC + i);
+              acc[h][i] += b.x; acc[h][i + 1] += b.y; acc[h][i + 2] += b.z; acc[h][i + 3] += b.w;
+            }
           }
+          if (p.row_scale) {
 #pragma unroll
-          for (int i = 0; i < NC; ++i) acc[h][i] *= rs;
+            for (int i = 0; i < NC; ++i) acc[h][i] *= rs;
+          }
           if (staged) {
             if (p.out_dtype == SB_F32) {
               if (h == 1) {
@@ -555,21 +650,24 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           for (int b = 0; b < kBlocks; ++b) {
             const int c0 = w.n0 + b * C::kHalf + part * NC;
             const int valid = p.n - c0;
-            const float* bias = p.bias ? p.bias + w.g * p.bias_group + c0 : nullptr;
-            const float* bgate = kGate && p.bias_gate ? p.bias_gate + w.g * p.bias_group + c0 : nullptr;
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
-              float y;
+            for (int i = 0; i < NC; i += 4) {
+              const float4 b0 = *reinterpret_cast<const float4*>(s_bs + b * NC + i);  // SwiGLU: of the gate
+              const float bv[4] = {b0.x, b0.y, b0.z, b0.w};
+              float uv[4] = {0.f, 0.f, 0.f, 0.f};
               if (kGate) {
-                const float up = acc[1][i] + (bias && i < valid ? bias[i] : 0.f);
-                y = silu_bf16out(acc[0][i] + (bgate && i < valid ? bgate[i] : 0.f)) * up;
-              } else {
-                y = gelu_bf16out(acc[b][i] + (bias && i < valid ? bias[i] : 0.f));
+                const float4 b1 = *reinterpret_cast<const float4*>(s_bs + NC + i);
+                uv[0] = b1.x; uv[1] = b1.y; uv[2] = b1.z; uv[3] = b1.w;
               }
-              y = i < valid ? y : 0.f;
-              acc[b][i] = y;
-              m = max(m, abs_bits(y));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float y = acc[b][i + j] + bv[j];
+                y = kGate ? silu_bf16out(y) * (acc[1][i + j] + uv[j]) : gelu_bf16out(y);
+                y = i + j < valid ? y : 0.f;
+                acc[b][i + j] = y;
+                m = max(m, abs_bits(y));
+              }
             }
             s_max[(b * C::kParts + part) * C::kBM + r] = m;
           }
@@ -635,7 +733,8 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 // whose partial sums are added in rank order through distributed shared memory:
 // one launch, no workspace, the same result every time.
 //
-// Warps: 0-7 epilogue (quarter w % 4, columns half w / 4), 8 TMA, 9 MMA (+TMEM).
+// Warps: 0-7 epilogue (quarter w % 4, columns half w / 4), 8 TMA, 9 MMA (+TMEM),
+// 10 scales (as in the kernel above).
 template <int EPI, int kN>
 struct F8DecCfg {
   static constexpr bool kGate = EPI == SB_EPI_SWIGLU;
@@ -648,18 +747,19 @@ struct F8DecCfg {
   static constexpr int kAcc = 4;  // accumulators in flight between the MMAs and the epilogue
   static constexpr int kAccCols = kTiles * kN;
   static constexpr int kTmemCols = kAcc * kAccCols < 32 ? 32 : kAcc * kAccCols;
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 352;
   static constexpr int kCols = kN / 2;  // columns per epilogue thread and tile
   static constexpr int kOffX = kStages * kTiles * kWBytes;
   static constexpr int kOffBar = kOffX + kStages * kXBytes;
-  static constexpr int kOffMisc = kOffBar + (2 * kStages + 2 * kAcc) * 8;
-  static constexpr int kOffFactor = (kOffMisc + 16 + 15) / 16 * 16;        // float [8 warps][kTiles][kCols]
-  static constexpr int kOffMax = kOffFactor + 8 * kTiles * kCols * 4;      // uint32 [kN][4 quarters]
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + kAcc) * 8;
+  static constexpr int kOffScale = (kOffMisc + 16 + 15) / 16 * 16;         // float [kAcc][kTiles][kN]
+  static constexpr int kOffMax = kOffScale + kAcc * kTiles * kN * 4;       // uint32 [kN][4 quarters]
   static constexpr int kOffPrefix = kOffMax + kN * 4 * 4;
   static constexpr int kOffOffsets = kOffPrefix + (kF8MaxG + 1) * 4;
   static constexpr int kSmemBytes = kOffOffsets + (kF8MaxG + 1) * 4 + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(kTmemCols <= 512, "accumulators");
+  static_assert(kStages >= kAcc, "a stage's barrier is waited for before its next use completes");
   static_assert(kTiles * kN * 128 * 4 <= kOffX, "the split's partial sums reuse the weight stages");
 };
 
@@ -717,14 +817,14 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* empty = full + S;
-  uint64_t* acc_full = empty + S;
-  uint64_t* acc_empty = acc_full + C::kAcc;
+  uint64_t* done = full + S;  // stage free and accumulator complete (S >= kAcc)
+  uint64_t* acc_empty = done + S;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
   const int rank = static_cast<int>(blockIdx.x) % splits;  // splits == cluster size
   const int first = static_cast<int>(blockIdx.x) / splits, stride = static_cast<int>(gridDim.x) / splits;
   const int G = p.num_groups;
@@ -734,13 +834,10 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   const int nk = static_cast<int>(static_cast<int64_t>(nk_all) * (rank + 1) / splits) - kb0;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&full[s], 2);  // the copies, and the scale warp
+      mbar_init(&done[s], 1);
     }
-    for (int b = 0; b < C::kAcc; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
-    }
+    for (int b = 0; b < C::kAcc; ++b) mbar_init(&acc_empty[b], 8);
     fence_barrier_init();
   }
   if (warp == 8 && lane == 0) {
@@ -786,95 +883,120 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
 
   if (warp == 8) {
     // ---------------------------------------------------------------- TMA
-    if (lane == 0) {
-      int it = 0;
+    if (elect_one()) {
+      Ring<S> st;
+      int issued = 0;
       for (int t = first; t < total && ok; t += stride) {
         const F8Item w = f8_dec_item<kN>(prefix, s_off, G, n_tiles, p.max_rows, t);
         const int wrow = static_cast<int>(w.g * p.b_group_rows) + w.n0;
-        for (int kk = 0; kk < nk; ++kk, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
-          mbar_expect_tx(&full[s], C::kStageBytes);
+        for (int kk = 0; kk < nk; ++kk, st.next()) {
+          uint64_t* const bar = &full[st.slot];
+          if (!mbar_wait(&done[st.slot], st.parity ^ 1, p.status, SB_DEVERR_MMA_WAIT)) { ok = false; break; }
+          if (issued < S) ++issued;
+          mbar_expect_tx(bar, C::kStageBytes);
           const int k0 = (kb0 + kk) * 128;
-          uint8_t* wdst = smem + s * NT * C::kWBytes;
-          if (kGate) tma_load_2d(wdst, &tmG, &full[s], k0, wrow);
-          tma_load_2d(wdst + (NT - 1) * C::kWBytes, &tmW, &full[s], k0, wrow);
-          tma_load_2d(smem + C::kOffX + s * C::kXBytes, &tmX, &full[s], k0, w.row0);
+          uint8_t* wdst = smem + st.slot * NT * C::kWBytes;
+          if (kGate) tma_load_2d(wdst, &tmG, bar, k0, wrow);
+          tma_load_2d(wdst + (NT - 1) * C::kWBytes, &tmW, bar, k0, wrow);
+          tma_load_2d(smem + C::kOffX + st.slot * C::kXBytes, &tmX, bar, k0, w.row0);
         }
       }
-      for (int i = it - S > 0 ? it - S : 0; i < it; ++i)
-        if (!mbar_wait(&empty[i % S], (i / S) & 1, p.status, SB_DEVERR_DRAIN)) break;
+      for (int i = 0; i < issued; ++i, st.next()) {
+        const int slot = (st.slot + S - issued) % S;
+        if (!mbar_wait(&done[slot], (st.slot >= issued ? st.parity : st.parity ^ 1), p.status, SB_DEVERR_DRAIN)) break;
+      }
     }
     __syncwarp();
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = idesc_e4m3_f32(128, kN);
-      int it = 0;
+      Ring<S> st;
+      Ring<C::kAcc> acc;
+      const uint32_t w_lo = f8_desc_lo(smem_u32(smem)), x_lo = f8_desc_lo(smem_u32(smem + C::kOffX));
       for (int t = first; t < total && ok; t += stride) {
-        for (int kk = 0; kk < nk; ++kk, ++it) {
-          const int s = it % S, buf = it % C::kAcc;
-          ok = mbar_wait(&acc_empty[buf], ((it / C::kAcc) & 1) ^ 1, p.status, SB_DEVERR_EPI_WAIT) &&
-               mbar_wait(&full[s], (it / S) & 1, p.status, SB_DEVERR_TMA_WAIT);
-          if (!ok) break;
+        for (int kk = 0; kk < nk; ++kk, st.next(), acc.next()) {
+          if (!mbar_wait(&full[st.slot], st.parity, p.status, SB_DEVERR_TMA_WAIT)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t w_base = smem_u32(smem + s * NT * C::kWBytes);
-          const uint32_t x_base = smem_u32(smem + C::kOffX + s * C::kXBytes);
+          const uint32_t wl = w_lo + st.slot * (NT * C::kWBytes >> 4), xl = x_lo + st.slot * (C::kXBytes >> 4);
 #pragma unroll
           for (int h = 0; h < NT; ++h)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              tc_mma_f8<false>(tmem + buf * C::kAccCols + h * kN, smem_desc_k_sw128(w_base + h * C::kWBytes + q * 32),
-                               smem_desc_k_sw128(x_base + q * 32), idesc, q > 0);
-          tc_commit(&empty[s]);
-          tc_commit(&acc_full[buf]);
+              tc_mma_f8<false>(tmem + acc.slot * C::kAccCols + h * kN, f8_desc(wl + h * (C::kWBytes >> 4) + 2 * q),
+                               f8_desc(xl + 2 * q), idesc, q > 0);
+          tc_commit(&done[st.slot]);
         }
       }
     }
     __syncwarp();
+  } else if (warp == 10) {
+    // ---------------------------------------------------------------- scales
+    Ring<S> st;
+    Ring<C::kAcc> acc;
+    constexpr int kAhead = 4, kX = (kN + 31) / 32;
+    for (int t = first; t < total && ok; t += stride) {
+      const F8Item w = f8_dec_item<kN>(prefix, s_off, G, n_tiles, p.max_rows, t);
+      const float* sa_ptr = p.a_scale + static_cast<int64_t>(w.row0 + lane) * p.a_scale_row + kb0 * p.a_scale_block;
+      const int64_t wofs = w.g * p.b_scale_group + (w.n0 / 128) * p.b_scale_row + kb0 * p.b_scale_block;
+      const float* sw_ptr = p.b_scale + wofs;
+      const float* sg_ptr = kGate ? p.b_gate_scale + wofs : nullptr;
+      float sa[kAhead][kX], sw[kAhead], sg[kAhead];
+      auto load = [&](int kk, int i) {
+        if (kk >= nk) return;
+#pragma unroll
+        for (int j = 0; j < kX; ++j)
+          sa[i][j] = lane + 32 * j < w.rows ? *sa_ptr_at(sa_ptr, j, p.a_scale_row, kk, p.a_scale_block) : 0.f;
+        sw[i] = sw_ptr[kk * p.b_scale_block];
+        if (kGate) sg[i] = sg_ptr[kk * p.b_scale_block];
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) load(i, i);
+      for (int kk0 = 0; kk0 < nk && ok; kk0 += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (kk0 + i >= nk) break;
+          if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[acc.slot], acc.parity ^ 1, p.status, SB_DEVERR_EPI_WAIT))) {
+            ok = false;
+            break;
+          }
+          float* f = reinterpret_cast<float*>(smem + C::kOffScale) + acc.slot * NT * kN;
+#pragma unroll
+          for (int j = 0; j < kX; ++j)
+            if (lane + 32 * j < kN) {
+              if (kGate) f[lane + 32 * j] = sa[i][j] * sg[i];
+              f[(NT - 1) * kN + lane + 32 * j] = sa[i][j] * sw[i];
+            }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[st.slot]);
+          st.next();
+          acc.next();
+          load(kk0 + i + kAhead, i);
+        }
+      }
+    }
   } else {
     // ---------------------------------------------------------------- epilogue
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * NC;
-    float* s_f = reinterpret_cast<float*>(smem + C::kOffFactor) + warp * NT * NC;
+    const float* s_f = reinterpret_cast<const float*>(smem + C::kOffScale) + half * NC;
     uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
     float* s_red = reinterpret_cast<float*>(smem);  // [kN][128], splits > 1 only
-    int it = 0;
+    Ring<S> st;
+    Ring<C::kAcc> ring_acc;
     for (int t = first; t < total && ok; t += stride) {
       const F8Item w = f8_dec_item<kN>(prefix, s_off, G, n_tiles, p.max_rows, t);
       const int feat = w.n0 + quarter * 32 + lane;
       const bool fvalid = feat < p.n;
       const bool warp_live = half * NC < w.rows;  // some token column of this warp is valid
-      // lane i (mod NC) stages the factors of column i of each tile
-      const int scol = half * NC + lane % NC;
-      const bool sc_live = lane < NC && scol < w.rows;
-      const float* sa_ptr = p.a_scale + static_cast<int64_t>(w.row0 + (sc_live ? scol : 0)) * p.a_scale_row +
-                            kb0 * p.a_scale_block;
-      const int64_t wofs = w.g * p.b_scale_group + (w.n0 / 128) * p.b_scale_row + kb0 * p.b_scale_block;
-      const float* sw_ptr = p.b_scale + wofs;
-      const float* sg_ptr = kGate ? p.b_gate_scale + wofs : nullptr;
       uint64_t sum[NT][NC / 2];
 #pragma unroll
       for (int h = 0; h < NT; ++h)
 #pragma unroll
         for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
-      float sa = 0.f, sw = 0.f, sg = 0.f;
-      auto load_scales = [&](int kk) {
-        if (sc_live) sa = sa_ptr[kk * p.a_scale_block];
-        sw = sw_ptr[kk * p.b_scale_block];
-        if (kGate) sg = sg_ptr[kk * p.b_scale_block];
-      };
-      if (nk > 0) load_scales(0);
-      for (int kk = 0; kk < nk; ++kk, ++it) {
-        const int buf = it % C::kAcc;
-        __syncwarp();
-        if (lane < NC) {
-          if (kGate) s_f[lane] = sa * sg;
-          s_f[(NT - 1) * NC + lane] = sa * sw;
-        }
-        __syncwarp();
-        if (kk + 1 < nk) load_scales(kk + 1);
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it / C::kAcc) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
+      for (int kk = 0; kk < nk; ++kk, st.next(), ring_acc.next()) {
+        const int buf = ring_acc.slot;
+        if (!__all_sync(0xffffffffu, mbar_wait(&done[st.slot], st.parity, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
@@ -884,23 +1006,17 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
           for (int h = 0; h < NT; ++h) {
             uint64_t v[NC / 2];
             tmem_ld_cols<NC>(lane_addr + buf * C::kAccCols + h * kN, v);
-            if (h == NT - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&acc_empty[buf]);
-            }
 #pragma unroll
             for (int i = 0; i < NC / 2; i += 2) {
-              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + h * NC + 2 * i);
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s_f + buf * NT * kN + h * kN + 2 * i);
               fma_pair(sum[h][i], v[i], f.x);
               fma_pair(sum[h][i + 1], v[i + 1], f.y);
             }
           }
-        } else {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
       }
       float acc[NT][NC];
 #pragma unroll
