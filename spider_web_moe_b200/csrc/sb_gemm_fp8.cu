@@ -23,11 +23,12 @@
 // rows of a and half of the weight rows, which halves the weight traffic into
 // shared memory, the limit of the one-CTA tile.
 //
-// Scales come through shared memory from a warp of their own: a block's scales
-// are loaded two blocks ahead, multiplied, and written to the slot of the
-// accumulator they belong to once that accumulator was read.  The same arrival
-// tells the MMA thread that the accumulator is free, so it waits for one barrier
-// per block, full (operands landed, accumulator free), and signals one, done.
+// Scales come through shared memory from a warp of their own, which works up to
+// four blocks ahead: it loads a block's scales, multiplies them, writes them to
+// one of four slots and arrives on the block's full barrier, so that the epilogue,
+// which waits for the MMAs (done), finds both.  The epilogue's one arrival per
+// block (released) frees the accumulator for the MMAs two blocks on and the scale
+// slot for the scale warp four blocks on.
 //
 // Warps: 0-7 epilogue (TMEM lane quarter w % 4, columns part w / 4), 8 TMA, 9
 // MMA (+TMEM), 10 scales.  Every wait is bounded (sb_common.cuh); loads use no
@@ -55,7 +56,6 @@ struct F8Cfg {
   static constexpr int kParts = 2;                     // epilogue warps per TMEM lane quarter
   static constexpr int kCols = kHalf / kParts;         // columns of each half per epilogue thread
   static constexpr int kEpiWarps = 4 * kParts;
-  static constexpr int kChunk = 32;                    // columns per TMEM load
   static constexpr int kThreads = (kEpiWarps + 4) * 32;  // whole warpgroups: registers move between them
   // Registers per thread at launch (65536 / kThreads, in steps of 8) and after
   // the split.
@@ -68,17 +68,21 @@ struct F8Cfg {
   static constexpr int kBoxBytes = 32 * 128;
   static constexpr int kOffOut = kOffB + kStages * kBBytes;
   static constexpr int kOffBar = kOffOut + (kPair ? kEpiWarps * 2 * kBoxBytes : 0);
-  static constexpr int kOffMisc = kOffBar + (2 * kStages + 2) * 8;
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + 4) * 8;
   static constexpr int kOffMax = (kOffMisc + 64 + 15) / 16 * 16;                            // uint32 [2 blocks][kParts][128 rows]
-  static constexpr int kOffBias = kOffMax + 2 * kParts * kBM * 4;          // float [warps][2][kCols]
-  static constexpr int kOffScale = kOffBias + kEpiWarps * 2 * kCols * 4;   // float [2 accumulators][kScaleFloats]
+  // What the epilogue needs once per item, from the scale warp: bias of the tile's
+  // 256 columns, row scale of its 128 rows.  The scale warp is at most four blocks,
+  // so at most four items, ahead of the item whose epilogue runs.
+  static constexpr int kItemSlots = 8, kItemFloats = 2 * kHalf + kBM;
+  static constexpr int kOffItem = kOffMax + 2 * kParts * kBM * 4;          // float [kItemSlots][kItemFloats]
+  static constexpr int kOffScale = kOffItem + kItemSlots * kItemFloats * 4;  // float [4 blocks][kScaleFloats]
   static constexpr int kScaleFloats = kBM + 2 * kHalf;  // [2][128 rows] products, or [128] a and [256] b (kBRows)
-  static constexpr int kOffPrefix = kOffScale + 2 * kScaleFloats * 4;      // int [kF8MaxG + 1]
+  static constexpr int kOffPrefix = kOffScale + 4 * kScaleFloats * 4;      // int [kF8MaxG + 1]
   static constexpr int kOffOffsets = kOffPrefix + (kF8MaxG + 1) * 4;
   static constexpr int kSmemBytes = kOffOffsets + (kF8MaxG + 1) * 4 + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(kTmemCols == 512, "two accumulators of 256 columns");
-  static_assert(kOffBias % 16 == 0 && kOffScale % 16 == 0, "16-byte reads");
+  static_assert(kOffItem % 16 == 0 && kOffScale % 16 == 0, "16-byte reads");
 };
 
 // Instruction descriptor: e4m3 x e4m3 -> fp32, both K-major, M x N tile.
@@ -151,16 +155,14 @@ template <int kN>
 SB_DEVINL void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[kN / 2]) {
   static_assert(kN == 16 || kN == 32, "x16 or x32 loads");
   uint32_t r[kN];
+#define SB_R8(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
   if constexpr (kN == 32)
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : SB_R8(0), SB_R8(8), SB_R8(16), SB_R8(24)
         : "r"(taddr)
         : "memory");
   else
@@ -168,10 +170,10 @@ SB_DEVINL void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[kN / 2]) {
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : SB_R8(0), SB_R8(8)
         : "r"(taddr)
         : "memory");
+#undef SB_R8
 #pragma unroll
   for (int i = 0; i < kN / 2; ++i) asm("mov.b64 %0, {%1, %2};" : "=l"(v[i]) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
 }
@@ -181,6 +183,31 @@ SB_DEVINL void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[kN / 2]) {
 // once per block of k (16384 x 4096 x 8192: 1190 us with it, 685 us without).
 SB_DEVINL void mbar_arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Two loads of 32 columns in flight, each in the registers after tmem_wait.
+struct Cols32 {
+  uint32_t r[32];
+};
+#define SB_R8(M, r, i) M(r[i]), M(r[i + 1]), M(r[i + 2]), M(r[i + 3]), M(r[i + 4]), M(r[i + 5]), M(r[i + 6]), M(r[i + 7])
+SB_DEVINL void tmem_start32(uint32_t taddr, Cols32& c) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : SB_R8("=r", c.r, 0), SB_R8("=r", c.r, 8), SB_R8("=r", c.r, 16), SB_R8("=r", c.r, 24)
+      : "r"(taddr)
+      : "memory");
+}
+SB_DEVINL void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Keeps uses of c behind the tmem_wait before it.
+SB_DEVINL void tmem_landed(Cols32& c) {
+  asm volatile("" : SB_R8("+r", c.r, 0), SB_R8("+r", c.r, 8), SB_R8("+r", c.r, 16), SB_R8("+r", c.r, 24));
+}
+#undef SB_R8
+SB_DEVINL uint64_t pair_at(const Cols32& c, int i) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(c.r[2 * i]), "r"(c.r[2 * i + 1]));
+  return v;
 }
 SB_DEVINL uint64_t pair_of(float x) {
   uint64_t r;
@@ -271,9 +298,11 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // a pair uses the leader's
   // A block's MMAs are done: its stage is free and its accumulator is complete.
-  // (S >= 2: the MMAs of the stage's next use wait for acc_empty of this one.)
+  // (The MMAs of the stage's next use wait until every warp has waited for this one.)
   uint64_t* done = full + S;
-  uint64_t* acc_empty = done + S;  // [2]: this CTA's epilogue has read accumulator and scales
+  // [4], by block: the epilogue has read the accumulator and the scales.  The
+  // leader's of a pair counts both CTAs' warps.
+  uint64_t* released = done + S;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
@@ -291,7 +320,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       mbar_init(&full[s], 1 + (kPair ? 2 : 1));  // the copies, and each CTA's scale warp
       mbar_init(&done[s], 1);
     }
-    for (int b = 0; b < 2; ++b) mbar_init(&acc_empty[b], C::kEpiWarps);
+    for (int b = 0; b < 4; ++b) mbar_init(&released[b], C::kEpiWarps * (kPair && rank == 0 ? 2 : 1));
     fence_barrier_init();
   }
   if (warp == kTmaWarp && lane == 0) {
@@ -401,14 +430,17 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       if (rank == 0 && elect_one()) {
         Ring<S> st;
         Ring<2> acc;
+        Ring<4> rel{2, 1};  // of the block two back
         const uint32_t a_lo = f8_desc_lo(smem_u32(smem + C::kOffA)), b_lo = f8_desc_lo(smem_u32(smem + C::kOffB));
         bool ok = true;
         for (int t = first; t < total && ok; t += stride) {
           const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
           const bool second = kGate || w.n0 + C::kHalf < p.n;
           const uint32_t idesc = idesc_e4m3_f32(C::kItemRows, second ? 2 * C::kHalf : C::kHalf);
-          for (int kk = 0; kk < nk; ++kk, st.next(), acc.next()) {
-            if (!mbar_wait(&full[st.slot], st.parity, p.status, SB_DEVERR_TMA_WAIT)) { ok = false; break; }
+          for (int kk = 0; kk < nk; ++kk, st.next(), acc.next(), rel.next()) {
+            ok = mbar_wait(&released[rel.slot], rel.parity, p.status, SB_DEVERR_EPI_WAIT) &&
+                 mbar_wait(&full[st.slot], st.parity, p.status, SB_DEVERR_TMA_WAIT);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t al = a_lo + st.slot * (C::kABytes >> 4), bl = b_lo + st.slot * (C::kBBytes >> 4);
 #pragma unroll
@@ -423,9 +455,10 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     } else if (warp == kScaleWarp) {
       // ---------------------------------------------------------------- scales
       Ring<S> st;
-      Ring<2> acc;
+      Ring<4> rel;
+      int item = 0;
       bool ok = true;
-      for (int t = first; t < total && ok; t += stride) {
+      for (int t = first; t < total && ok; t += stride, item = (item + 1) % C::kItemSlots) {
         const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
         const bool second = kGate || w.n0 + C::kHalf < p.n;
         const float* sa_ptr = p.a_scale + static_cast<int64_t>(w.row0 + lane) * p.a_scale_row;
@@ -437,7 +470,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         } else {
           sb1 += static_cast<int64_t>(w.n0 + lane) * p.b_scale_row;
         }
-        constexpr int kAhead = 2, kB = kBRows ? 8 : 2;
+        constexpr int kAhead = kBRows ? 1 : 2, kB = kBRows ? 8 : 2;
         float sa[kAhead][4], sb[kAhead][kB];
         auto load = [&](int kk, int i) {
           if (kk >= nk) return;
@@ -460,11 +493,24 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
           for (int i = 0; i < kAhead; ++i) {
             if (kk0 + i >= nk) break;
-            if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[acc.slot], acc.parity ^ 1, p.status, SB_DEVERR_EPI_WAIT))) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&released[rel.slot], rel.parity ^ 1, p.status, SB_DEVERR_EPI_WAIT))) {
               ok = false;
               break;
             }
-            float* f = reinterpret_cast<float*>(smem + C::kOffScale) + acc.slot * C::kScaleFloats;
+            if (i == 0 && kk0 == 0) {
+              float* d = reinterpret_cast<float*>(smem + C::kOffItem) + item * C::kItemFloats;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float* bias = kGate && j < 4 ? p.bias_gate : p.bias;
+                const int c = w.n0 + lane + 32 * (kGate ? j % 4 : j);
+                d[lane + 32 * j] = bias && c < p.n ? bias[w.g * p.bias_group + c] : 0.f;
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                d[2 * C::kHalf + lane + 32 * j] =
+                    p.row_scale && lane + 32 * j < w.rows ? p.row_scale[w.row0 + lane + 32 * j] : 1.f;
+            }
+            float* f = reinterpret_cast<float*>(smem + C::kOffScale) + rel.slot * C::kScaleFloats;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               f[lane + 32 * j] = kBRows ? sa[i][j] : sa[i][j] * sb[i][0];
@@ -480,7 +526,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               else mbar_arrive(&full[st.slot]);
             }
             st.next();
-            acc.next();
+            rel.next();
             load(kk0 + i + kAhead, i);
           }
         }
@@ -493,80 +539,104 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const int quarter = warp & 3, part = warp >> 2;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * NC;
     uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
-    float* s_bs = reinterpret_cast<float*>(smem + C::kOffBias) + warp * 2 * NC;
+    const uint32_t released_lead = kPair && rank != 0 ? mapa_shared(smem_u32(released), 0) : 0;
     Ring<S> st;
-    int buf = 0;
+    Ring<4> rel;
+    int item = 0;
     bool ok = true;
-    for (int t = first; t < total && ok; t += stride) {
-      const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
-      const int r = quarter * 32 + lane;          // row of this CTA's tile
-      const bool live = r < w.rows;
-      const bool warp_live = quarter * 32 < w.rows;
-      const bool second = kGate || w.n0 + C::kHalf < p.n;
-      const int64_t row = w.row0 + r;
-      // this lane's share of the warp's 2 NC bias values
-      constexpr int NB = NC / 16;
-      const int bcol = w.n0 + (lane >> 4) * C::kHalf + part * NC + (lane & 15) * NB;
+    for (int t = first; t < total && ok; t += stride, item = (item + 1) % C::kItemSlots) {
+      bool warp_live, second;
+      {
+        const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
+        warp_live = quarter * 32 < w.rows;
+        second = kGate || w.n0 + C::kHalf < p.n;
+      }
+      const int r = quarter * 32 + lane;  // row of this CTA's tile
       uint64_t sum[2][NC / 2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
-      // 0 without a bias, and past n; staged below once the sums are complete
-      float pbias[NB];
-      {
-        const float* bias = kGate && lane < 16 ? p.bias_gate : p.bias;
-        const int c0 = kGate ? w.n0 + part * NC + (lane & 15) * NB : bcol;
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-          pbias[j] = bias && c0 + j < p.n ? bias[w.g * p.bias_group + c0 + j] : 0.f;
-      }
-      for (int kk = 0; kk < nk; ++kk, st.next(), buf ^= 1) {
+      for (int kk = 0; kk < nk; ++kk, st.next(), rel.next()) {
+        const int buf = rel.slot & 1;
         if (!__all_sync(0xffffffffu, mbar_wait(&done[st.slot], st.parity, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t t0 = lane_addr + buf * C::kAccCols;
-        const float* f = reinterpret_cast<const float*>(smem + C::kOffScale) + buf * C::kScaleFloats;
+        const float* f = reinterpret_cast<const float*>(smem + C::kOffScale) + rel.slot * C::kScaleFloats;
         const uint64_t s0 = pair_of(f[r]), s1 = kBRows ? s0 : pair_of(f[C::kBM + r]);
-        constexpr int CH = C::kChunk;
-        constexpr int kLoads = 2 * NC / CH;
-        uint64_t v[CH / 2];
-        auto load = [&](int j) { tmem_ld_pairs<CH>(t0 + (j * CH / NC) * C::kHalf + j * CH % NC, v); };
-        auto add = [&](int j) {
-          const int h = j * CH / NC, c = j * CH % NC;
+        // columns 32 j .. of the warp's 2 x 64: two loads in flight, the second
+        // pair over the first pair's additions
+        auto add = [&](const Cols32& v, int j) {
+          const int h = j >> 1, c = (j & 1) * 32;
 #pragma unroll
-          for (int i = 0; i < CH / 2; i += 2) {
+          for (int i = 0; i < 16; i += 2) {
             if (kBRows) {
               const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(f + C::kBM + h * C::kHalf + part * NC + c + 2 * i);
-              fma_pair(sum[h][c / 2 + i], mul_pair(v[i], b.x), s0);
-              fma_pair(sum[h][c / 2 + i + 1], mul_pair(v[i + 1], b.y), s0);
+              fma_pair(sum[h][c / 2 + i], mul_pair(pair_at(v, i), b.x), s0);
+              fma_pair(sum[h][c / 2 + i + 1], mul_pair(pair_at(v, i + 1), b.y), s0);
             } else {
-              fma_pair(sum[h][c / 2 + i], v[i], h ? s1 : s0);
-              fma_pair(sum[h][c / 2 + i + 1], v[i + 1], h ? s1 : s0);
+              fma_pair(sum[h][c / 2 + i], pair_at(v, i), h ? s1 : s0);
+              fma_pair(sum[h][c / 2 + i + 1], pair_at(v, i + 1), h ? s1 : s0);
             }
           }
         };
-        if (warp_live) {
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&released[rel.slot]);
+            if (kPair && rank != 0) mbar_arrive_leader(released_lead + 8u * rel.slot);
+          }
+        };
+        if (warp_live && kBRows) {
+          // one load at a time: the scales of the columns need the registers
+          Cols32 v;
 #pragma unroll
-          for (int j = 0; j < kLoads - 1; ++j)
-            if (j * CH < NC || second) {
-              load(j);
-              add(j);
+          for (int j = 0; j < 4; ++j)
+            if (j < 2 || second) {
+              tmem_start32(t0 + (j >> 1) * C::kHalf + (j & 1) * 32, v);
+              tmem_wait();
+              tmem_landed(v);
+              add(v, j);
             }
-          if (second) load(kLoads - 1);
-          if (kBRows && second) add(kLoads - 1);  // reads the slot's scales
+          release();  // only now: add reads the slot's scales
+        } else if (warp_live) {
+          Cols32 va, vb;
+          tmem_start32(t0, va);
+          tmem_start32(t0 + 32, vb);
+          tmem_wait();
+          tmem_landed(va);
+          tmem_landed(vb);
+          if (second) {
+            add(va, 0);
+            tmem_start32(t0 + C::kHalf, va);
+            add(vb, 1);
+            tmem_start32(t0 + C::kHalf + 32, vb);
+            tmem_wait();
+            tmem_landed(va);
+            tmem_landed(vb);
+            release();
+            add(va, 2);
+            add(vb, 3);
+          } else {
+            add(va, 0);
+            add(vb, 1);
+            release();
+          }
+        } else {
+          release();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        if (!kBRows && warp_live && second) add(kLoads - 1);
       }
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < NB; ++j) s_bs[lane * NB + j] = pbias[j];
-      __syncwarp();
+      // the item again, so that its fields need no registers beside the sums
+      int t_again = t;
+      asm volatile("" : "+r"(t_again));
+      const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t_again, rank);
+      const bool live = r < w.rows;
+      const int64_t row = w.row0 + r;
+      const float* s_bias = reinterpret_cast<const float*>(smem + C::kOffItem) + item * C::kItemFloats + part * NC;
       float acc[2][NC];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -575,7 +645,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[h][2 * i]), "=f"(acc[h][2 * i + 1]) : "l"(sum[h][i]));
       if constexpr (!kQuant) {
         if (!ok || !warp_live) continue;
-        const float rs = live && p.row_scale ? p.row_scale[row] : 1.f;
+        const float rs = s_bias[2 * C::kHalf - part * NC + r];
         // whole boxes of 32 rows leave through shared memory (the hardware clips
         // columns past n); element stores would keep the warp, and with it the
         // tensor core, waiting for 16-byte pieces of 32 different rows
@@ -593,7 +663,8 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           if (p.bias) {
 #pragma unroll
             for (int i = 0; i < NC; i += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(s_bs + h * NC + i);
+              if (i % 16 == 0) asm volatile("" ::: "memory");  // keeps the loads from piling up in registers
+              const float4 b = *reinterpret_cast<const float4*>(s_bias + h * C::kHalf + i);
               acc[h][i] += b.x; acc[h][i + 1] += b.y; acc[h][i + 2] += b.z; acc[h][i + 3] += b.w;
             }
           }
@@ -653,11 +724,12 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             uint32_t m = 0;
 #pragma unroll
             for (int i = 0; i < NC; i += 4) {
-              const float4 b0 = *reinterpret_cast<const float4*>(s_bs + b * NC + i);  // SwiGLU: of the gate
+              if (i % 16 == 0) asm volatile("" ::: "memory");  // keeps the loads from piling up in registers
+              const float4 b0 = *reinterpret_cast<const float4*>(s_bias + b * C::kHalf + i);  // SwiGLU: of the gate
               const float bv[4] = {b0.x, b0.y, b0.z, b0.w};
               float uv[4] = {0.f, 0.f, 0.f, 0.f};
               if (kGate) {
-                const float4 b1 = *reinterpret_cast<const float4*>(s_bs + NC + i);
+                const float4 b1 = *reinterpret_cast<const float4*>(s_bias + C::kHalf + i);
                 uv[0] = b1.x; uv[1] = b1.y; uv[2] = b1.z; uv[3] = b1.w;
               }
 #pragma unroll
