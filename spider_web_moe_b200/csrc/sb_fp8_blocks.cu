@@ -89,6 +89,76 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(const sb_fp8_qua
   }
 }
 
+// The same for bf16 rows on 16-byte boundaries with whole 8-column chunks: 8 lanes
+// hold a block, 16 elements each, as loaded (two elements per register): the
+// maximum of two is one 16-bit-pair instruction, two blocks share a register in
+// the shuffles, and the few registers leave room for more loads in flight.
+constexpr int kBf16Blocks = 4;
+
+__global__ void __launch_bounds__(256, 4) fp8_quantize_rows_bf16_kernel(const sb_fp8_quantize_args p) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane8 = threadIdx.x & 7;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
+  const int cb0 = blockIdx.y * kBf16Blocks;
+  int64_t rows = p.rows;
+  if (p.row_count) rows = min(rows, static_cast<int64_t>(*p.row_count));
+  const bool live = r < rows;
+  const int64_t src = live ? (p.row_index ? p.row_index[r] : r) : 0;
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + blockIdx.z * p.x_batch + src * p.x_row;
+  uint8_t* q = static_cast<uint8_t*>(p.q) + blockIdx.z * p.q_batch + r * p.ldq;
+  float* scale = p.scale + blockIdx.z * p.scale_batch + r * p.scale_row;
+  // a lane's 16 elements are 8 at lane8 * 8 and 8 at 64 + lane8 * 8: each load of
+  // the 8 lanes is 128 consecutive bytes
+  uint4 v[kBf16Blocks][2];
+#pragma unroll
+  for (int i = 0; i < kBf16Blocks; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = (cb0 + i) * 128 + h * 64 + lane8 * 8;
+      v[i][h] = live && c < p.cols ? *reinterpret_cast<const uint4*>(x + c) : make_uint4(0, 0, 0, 0);
+    }
+  uint32_t amax[kBf16Blocks];
+#pragma unroll
+  for (int i = 0; i < kBf16Blocks; i += 2) {
+    uint32_t m[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint4 a = v[i + k][0], b = v[i + k][1];
+      constexpr uint32_t kAbs = 0x7fff7fffu;
+      m[k] = __vmaxu2(__vmaxu2(__vmaxu2(a.x & kAbs, a.y & kAbs), __vmaxu2(a.z & kAbs, a.w & kAbs)),
+                      __vmaxu2(__vmaxu2(b.x & kAbs, b.y & kAbs), __vmaxu2(b.z & kAbs, b.w & kAbs)));
+    }
+    // low halves: block i, high halves: block i + 1
+    uint32_t w = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) w = __vmaxu2(w, __shfl_xor_sync(0xffffffffu, w, o));
+    amax[i] = w << 16;
+    amax[i + 1] = w & 0xffff0000u;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < kBf16Blocks; ++i) {
+    const int cb = cb0 + i;
+    if (cb * 128 >= p.cols) break;
+    const Fp8Scale s = fp8_scale(amax[i]);
+    if (lane8 == 0) scale[static_cast<int64_t>(cb) * p.scale_col] = s.scale;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = cb * 128 + h * 64 + lane8 * 8;
+      if (c >= p.cols) continue;
+      const uint32_t w[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = __uint_as_float(w[j] << 16) * s.inv;
+        f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * s.inv;
+      }
+      *reinterpret_cast<uint2*>(q + c) = make_uint2(fp8_pack4(f[0], f[1], f[2], f[3]), fp8_pack4(f[4], f[5], f[6], f[7]));
+    }
+  }
+}
+
 // ---------------------------------------------------------------- tiles
 // 128 x 128 tile per CTA through shared memory: block_rows 128 (one scale per
 // tile), and block_rows 1 of a matrix whose rows, not columns, are contiguous
@@ -193,6 +263,10 @@ static int quantize_typed(const sb_fp8_quantize_args& p, cudaStream_t st) {
   if (p.block_rows == 1 && (p.x_row != 1 || p.x_col == 1 || p.row_index)) {
     const dim3 grid((p.rows + kRowsPerCta - 1) / kRowsPerCta, (p.cols + 128 * kRowsBlocks - 1) / (128 * kRowsBlocks),
                     p.batch);
+    if (sizeof(T) == 2 && p.x_col == 1 && base && p.x_row % 8 == 0 && p.cols % 8 == 0)
+      return launch(fp8_quantize_rows_bf16_kernel,
+                    dim3((p.rows + 31) / 32, (p.cols + 128 * kBf16Blocks - 1) / (128 * kBf16Blocks), p.batch), dim3(256), 0,
+                    st, p);
     if (p.x_col == 1 && base && p.x_row % kAlign == 0)
       return launch(fp8_quantize_rows_kernel<T, true>, grid, dim3(256), 0, st, p);
     return launch(fp8_quantize_rows_kernel<T, false>, grid, dim3(256), 0, st, p);

@@ -1305,7 +1305,11 @@ static int launch_f8_decode(const sb_fp8_matmul_args& a, cudaStream_t st) {
 // schedule runs, and its column count.
 static int decode_columns(const sb_fp8_matmul_args& a) {
   if (a.b_block_rows != 128) return 0;
-  if (!a.offsets) return a.max_rows <= 16 ? 16 : (a.max_rows <= 32 ? 32 : (a.max_rows <= 64 ? 64 : 0));
+  if (!a.offsets) {
+    if (a.max_rows <= 32) return a.max_rows <= 16 ? 16 : 32;
+    // up to 128 rows, in tiles of 64, while their items do not fill the GPU
+    return a.max_rows <= 64 || (a.max_rows <= 128 && (a.n + 127) / 128 * 2 <= current_sm_count()) ? 64 : 0;
+  }
   const int per_group = a.max_rows / a.num_groups;
   return per_group <= 4 ? 16 : (per_group <= 20 ? 32 : (per_group <= 48 ? 64 : 0));
 }
