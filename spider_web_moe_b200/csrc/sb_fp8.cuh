@@ -27,4 +27,10 @@ SB_DEVINL uint32_t fp8_pack4(float a, float b, float c, float d) {
   return lo | (hi << 16);
 }
 
+// Four bf16 values (two per word) times inv, to e4m3.
+SB_DEVINL uint32_t fp8_pack4_bf16(uint32_t a, uint32_t b, float inv) {
+  return fp8_pack4(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xffff0000u) * inv, __uint_as_float(b << 16) * inv,
+                   __uint_as_float(b & 0xffff0000u) * inv);
+}
+
 }  // namespace sb

@@ -147,14 +147,8 @@ __global__ void __launch_bounds__(256, 4) fp8_quantize_rows_bf16_kernel(const sb
     for (int h = 0; h < 2; ++h) {
       const int c = cb * 128 + h * 64 + lane8 * 8;
       if (c >= p.cols) continue;
-      const uint32_t w[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f[2 * j] = __uint_as_float(w[j] << 16) * s.inv;
-        f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * s.inv;
-      }
-      *reinterpret_cast<uint2*>(q + c) = make_uint2(fp8_pack4(f[0], f[1], f[2], f[3]), fp8_pack4(f[4], f[5], f[6], f[7]));
+      *reinterpret_cast<uint2*>(q + c) =
+          make_uint2(fp8_pack4_bf16(v[i][h].x, v[i][h].y, s.inv), fp8_pack4_bf16(v[i][h].z, v[i][h].w, s.inv));
     }
   }
 }
@@ -240,6 +234,130 @@ __global__ void __launch_bounds__(256) fp8_quantize_tile_kernel(const sb_fp8_qua
   }
 }
 
+// 128 x 128 blocks of bf16 rows on 16-byte boundaries (whole 8-column chunks): the
+// CTA's 8 x 16 bytes per thread stay in registers between the maximum and the
+// rounding; no tile in shared memory.
+__global__ void __launch_bounds__(256, 4) fp8_quantize_block_bf16_kernel(const sb_fp8_quantize_args p) {
+  __shared__ uint32_t s_max[8];
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane16 = tid & 15;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 128 + (tid >> 4);
+  const int c = blockIdx.x * 128 + lane16 * 8;
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + blockIdx.z * p.x_batch + c;
+  uint4 v[8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + 16 * i;
+    v[i] = r < p.rows && c < p.cols ? *reinterpret_cast<const uint4*>(x + r * p.x_row) : make_uint4(0, 0, 0, 0);
+  }
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    m = __vmaxu2(m, __vmaxu2(__vmaxu2(v[i].x & kAbs, v[i].y & kAbs), __vmaxu2(v[i].z & kAbs, v[i].w & kAbs)));
+  m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+  if ((tid & 31) == 0) s_max[tid >> 5] = m;
+  __syncthreads();
+  m = s_max[0];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) m = max(m, s_max[w]);
+  const Fp8Scale s = fp8_scale(m << 16);
+  if (tid == 0)
+    p.scale[blockIdx.z * p.scale_batch + blockIdx.y * p.scale_row + blockIdx.x * p.scale_col] = s.scale;
+  if (c >= p.cols) return;
+  uint8_t* q = static_cast<uint8_t*>(p.q) + blockIdx.z * p.q_batch + c;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + 16 * i;
+    if (r < p.rows) *reinterpret_cast<uint2*>(q + r * p.ldq) = make_uint2(fp8_pack4_bf16(v[i].x, v[i].y, s.inv), fp8_pack4_bf16(v[i].z, v[i].w, s.inv));
+  }
+}
+
+// bf16 matrices whose rows are contiguous (transposed views), rows a multiple of 8
+// and columns on 16-byte boundaries: the tile lies in shared memory as [col][row]
+// and a thread takes two neighbouring rows, one 32-bit word per column, and a
+// quarter of the columns.
+__global__ void __launch_bounds__(256, 4) fp8_quantize_transposed_bf16_kernel(const sb_fp8_quantize_args p) {
+  constexpr int kPitch = 136;  // elements; 68 words, so a warp's 32 row pairs meet no bank conflict
+  __shared__ __align__(16) __nv_bfloat16 tile[128 * kPitch];
+  __shared__ uint32_t s_max[256];
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 128;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 128;
+  const int nr = static_cast<int>(min(static_cast<int64_t>(128), p.rows - r0));
+  const int nc = static_cast<int>(min(static_cast<int64_t>(128), p.cols - c0));
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + blockIdx.z * p.x_batch + r0 + c0 * p.x_col;
+  {
+    const int r = (tid & 15) * 8;
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = i * 16 + (tid >> 4);
+      v[i] = r < nr && c < nc ? *reinterpret_cast<const uint4*>(x + c * p.x_col + r) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(tile + (i * 16 + (tid >> 4)) * kPitch + r) = v[i];
+  }
+  __syncthreads();
+  const int pair = tid & 63, quarter = tid >> 6;
+  uint32_t v[32];
+  uint32_t m = 0;
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    v[j] = *reinterpret_cast<const uint32_t*>(tile + (quarter * 32 + j) * kPitch + pair * 2);
+    m = __vmaxu2(m, v[j] & kAbs);
+  }
+  s_max[tid] = m;
+  __syncthreads();
+  float* scale = p.scale + blockIdx.z * p.scale_batch + blockIdx.x * p.scale_col;
+  float inv[2];
+  if (p.block_rows == 1) {
+    m = __vmaxu2(__vmaxu2(s_max[pair], s_max[pair + 64]), __vmaxu2(s_max[pair + 128], s_max[pair + 192]));
+    const Fp8Scale lo = fp8_scale(m << 16), hi = fp8_scale(m & 0xffff0000u);
+    inv[0] = lo.inv;
+    inv[1] = hi.inv;
+    if (quarter == 0 && pair * 2 < nr) {  // nr is even
+      scale[(r0 + pair * 2) * p.scale_row] = lo.scale;
+      scale[(r0 + pair * 2 + 1) * p.scale_row] = hi.scale;
+    }
+  } else {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, s_max[(tid & 31) + 32 * i]);
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    const Fp8Scale s = fp8_scale(m << 16);
+    inv[0] = inv[1] = s.inv;
+    if (tid == 0) scale[blockIdx.y * p.scale_row] = s.scale;
+  }
+  if (pair * 2 >= nr) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint8_t* q = static_cast<uint8_t*>(p.q) + blockIdx.z * p.q_batch + (r0 + pair * 2 + h) * p.ldq + c0 + quarter * 32;
+#pragma unroll
+    for (int j = 0; j < 32; j += 16) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t* u = v + j + 4 * k;
+        const uint32_t sel = h ? 0x7632 : 0x5410;
+        w[k] = fp8_pack4_bf16(__byte_perm(u[0], u[1], sel), __byte_perm(u[2], u[3], sel), inv[h]);
+      }
+      const int left = nc - quarter * 32 - j;
+      if (left >= 16) {
+        *reinterpret_cast<uint4*>(q + j) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < left) q[j + i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+      }
+    }
+  }
+}
+
 template <typename T, bool kColMajor, bool kVec>
 static int launch_tile(const sb_fp8_quantize_args& p, cudaStream_t st) {
   constexpr int kPitch = kColMajor ? 128 + 16 / sizeof(T) : 128 + 4 / sizeof(T);
@@ -272,6 +390,11 @@ static int quantize_typed(const sb_fp8_quantize_args& p, cudaStream_t st) {
     return launch(fp8_quantize_rows_kernel<T, false>, grid, dim3(256), 0, st, p);
   }
   if (p.rows > 65535 * 128) return SB_ERR_UNSUPPORTED;  // a grid's y extent
+  const dim3 tiles((p.cols + 127) / 128, (p.rows + 127) / 128, p.batch);
+  if (sizeof(T) == 2 && p.x_row == 1 && p.x_col != 1 && base && p.x_col % 8 == 0 && p.rows % 8 == 0)
+    return launch(fp8_quantize_transposed_bf16_kernel, tiles, dim3(256), 0, st, p);
+  if (sizeof(T) == 2 && p.x_col == 1 && base && p.x_row % 8 == 0 && p.cols % 8 == 0)
+    return launch(fp8_quantize_block_bf16_kernel, tiles, dim3(256), 0, st, p);
   if (p.x_row == 1 && p.x_col != 1)
     return base && p.x_col % kAlign == 0 ? launch_tile<T, true, true>(p, st) : launch_tile<T, true, false>(p, st);
   return p.x_col == 1 && base && p.x_row % kAlign == 0 ? launch_tile<T, false, true>(p, st)
