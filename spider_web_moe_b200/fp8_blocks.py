@@ -207,27 +207,27 @@ def _unit_cols(t: torch.Tensor) -> torch.Tensor:
 
 
 def _linear(x, weight, packed):
-    """y [M, N] for x [M, K] in one library call."""
+    """y [M, N] for x [M, K] in one library call (weight: the matrix, or the packed values)."""
     x = _unit_cols(x)
-    m, k = x.shape
-    dev = x.device
-    if packed is not None:
-        n, w, wcode, ldw, s = packed.q.shape[0], packed.q, L.SB_BF16, packed.pitch, packed.scale
-        sptr, srow, scol = s.data_ptr(), s.stride(0), s.stride(1)
-    else:
-        w = _unit_cols(weight)
-        n, wcode, ldw = w.shape[0], _DTYPES[w.dtype], max(w.stride(0), k)
-        sptr, srow, scol = None, 0, 0
-    y = torch.empty((m, n), dtype=x.dtype, device=dev)
+    (m, k), n = x.shape, weight.shape[0]
+    dev, code = x.device, _DTYPES[x.dtype]
+    y = x.new_empty((m, n))
     if m == 0 or n == 0:
         return y
     if k == 0:
         return y.zero_()
+    if packed is None:
+        w, s = _unit_cols(weight), None
+        warg = (w.data_ptr(), _DTYPES[w.dtype], max(w.stride(0), k), None, 0, 0)
+    else:
+        s = packed.scale
+        srow, scol = s.stride()
+        warg = (weight.data_ptr(), L.SB_BF16, packed.pitch, s.data_ptr(), srow, scol)
     lib = L.load()
     nbytes = lib.sb_fp8_linear_workspace_bytes(m, n, k, packed is not None)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    rc = L.on_device(dev, lib.sb_fp8_linear, x.data_ptr(), _DTYPES[x.dtype], max(x.stride(0), k), m, n, k, w.data_ptr(),
-                     wcode, ldw, sptr, srow, scol, y.data_ptr(), _status_ptr(dev), ws.data_ptr(), nbytes)
+    ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    rc = L.on_device(dev, lib.sb_fp8_linear, x.data_ptr(), code, max(x.stride(0), k), m, n, k, *warg, y.data_ptr(),
+                     _status_ptr(dev), ws.data_ptr(), nbytes)
     _finish(rc, "sb_fp8_linear", dev)
     return y
 
@@ -240,11 +240,12 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, packed):
         ctx.packed = packed
         ctx.save_for_backward(x, weight)
-        return _linear(x, weight, packed)
+        return _linear(x, weight if packed is None else packed.q, packed)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("fp8_block_linear is not twice differentiable")
         x, weight = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         if ctx.packed is not None:
@@ -272,25 +273,25 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
     and in a weight matrix; all three products run in fp8.  To capture a backward
     pass into a CUDA graph, drop eager graphs of the same leaves first: autograd
     ties their gradients to the stream those were built on."""
-    _dtype_code(x, "fp8_block_linear input")
     packed = weight if isinstance(weight, Fp8BlockTensor) else None
     w = weight if packed is None else packed.q
-    shape = w.shape
-    if len(shape) != 2 or x.dim() < 1 or x.shape[-1] != shape[1]:
-        raise ValueError(f"fp8_block_linear needs x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(shape)}")
+    if x.dtype not in _DTYPES or (packed is None and w.dtype not in _DTYPES):
+        raise TypeError(f"fp8_block_linear takes float32 or bfloat16, got {x.dtype} and {w.dtype}")
+    xs, ws = x.shape, w.shape
+    if len(ws) != 2 or not xs or xs[-1] != ws[1]:
+        raise ValueError(f"fp8_block_linear needs x [..., K] and weight [N, K], got {tuple(xs)} and {tuple(ws)}")
     if w.device != x.device:
         raise ValueError("x and weight must be on one device")
-    if packed is None:
-        _dtype_code(weight, "fp8_block_linear weight")
-    elif packed.block_rows != BLOCK:
+    if packed is not None and packed.block_rows != BLOCK:
         raise ValueError("packed weights need 128 x 128 blocks")
     _need_cuda(x, "fp8_block_linear")
-    x2 = x if x.dim() == 2 else x.reshape(-1, shape[1])
-    if torch.is_grad_enabled() and (x.requires_grad or (packed is None and weight.requires_grad)):
-        y = _Fp8Linear.apply(x2, None if packed is not None else weight, packed)
+    flat = len(xs) == 2
+    x2 = x if flat else x.reshape(-1, ws[1])
+    if torch.is_grad_enabled() and (x.requires_grad or (packed is None and w.requires_grad)):
+        y = _Fp8Linear.apply(x2, None if packed is not None else w, packed)
     else:
-        y = _linear(x2, weight, packed)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], shape[0])
+        y = _linear(x2, w, packed)
+    return y if flat else y.view(*xs[:-1], ws[0])
 
 
 class Fp8BlockExperts:

@@ -37,8 +37,8 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
 def _launch(logits, top_k, score, bias, num_groups, topk_groups, group_top, renormalize, scale):
     x = _rows(logits)
     n, e = x.shape
-    idx = torch.empty((n, top_k), dtype=torch.int32, device=x.device)
-    w = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
+    idx = x.new_empty((n, top_k), dtype=torch.int32)
+    w = x.new_empty((n, top_k), dtype=torch.float32)
     rc = L.on_device(x.device, L.load().sb_route_experts, x.data_ptr(), _dtype_code(x.dtype), max(x.stride(0), e), n,
                      e, top_k, score, L.ptr(bias), num_groups, topk_groups, group_top, renormalize, scale,
                      idx.data_ptr(), w.data_ptr())
@@ -60,17 +60,18 @@ class _RouteExperts(torch.autograd.Function):
         return idx, w
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, _, grad_w):
         if grad_w is None:
             return (None,) * 9
+        if torch.is_grad_enabled():
+            raise RuntimeError("route_experts is not twice differentiable")
         logits, idx, bias = ctx.saved_tensors
         score, renormalize, scale = ctx.args
         x = _rows(logits)
         n, e = x.shape
         k = idx.shape[-1]
         g = grad_w.reshape(n, k).to(torch.float32).contiguous()
-        dl = torch.empty((n, e), dtype=x.dtype, device=x.device)
+        dl = x.new_empty((n, e))
         rc = L.on_device(x.device, L.load().sb_route_experts_backward, x.data_ptr(), _dtype_code(x.dtype),
                          max(x.stride(0), e), n, e, k, score, L.ptr(bias), renormalize, scale, idx.data_ptr(),
                          g.data_ptr(), dl.data_ptr(), e)

@@ -294,6 +294,8 @@ def test_linear_shapes(cuda_device):
     xe = x[:0].clone().requires_grad_()
     fp8_block_linear(xe, wl).sum().backward()
     assert (wl.grad == 0).all() and xe.grad.shape == (0, 3, 64)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(fp8_block_linear(x, wl).sum(), wl, create_graph=True)
     # an expanded (stride 0) gradient, as sum() makes
     wl = w.clone().requires_grad_()
     fp8_block_linear(x, wl).float().sum().backward()

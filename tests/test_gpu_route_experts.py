@@ -215,6 +215,16 @@ def test_masked_rows_have_zero_gradient(cuda_device):
         assert (leaf.grad[0] == 0).all() and (leaf.grad[1, 1:] == 0).all()
 
 
+def test_not_twice_differentiable(cuda_device):
+    leaf = torch.randn(3, 8, device=cuda_device, requires_grad=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(route_experts(leaf, 2)[1].sum(), leaf, create_graph=True)
+    idx, w = route_experts(leaf, 2)
+    assert not idx.requires_grad and w.requires_grad
+    with torch.no_grad():
+        assert not route_experts(leaf, 2)[1].requires_grad
+
+
 def test_captured(cuda_device):
     g = torch.Generator().manual_seed(12)
     x = torch.randn(70, 64, generator=g).to(cuda_device)
