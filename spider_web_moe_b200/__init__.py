@@ -10,7 +10,9 @@ the synthetic-data helpers load without the CUDA library.
 from .config import ModelConfig, load_config  # noqa: F401
 
 __all__ = ["ModelConfig", "load_config", "SpiderMoELayer", "sparse_expert_delta", "LumenWorkspace",
-           "ExpertChunkStore", "CudaGraphDecodeRunner", "load_spiderw", "write_spiderw"]
+           "ExpertChunkStore", "CudaGraphDecodeRunner", "load_spiderw", "write_spiderw", "route_experts",
+           "quantize_fp8_blocks", "fp8_block_matmul", "fp8_block_linear", "fp8_expert_delta", "Fp8BlockTensor",
+           "Fp8BlockExperts"]
 
 _LAZY = {
     "SpiderMoELayer": ("layer", "SpiderMoELayer"),
@@ -20,6 +22,13 @@ _LAZY = {
     "CudaGraphDecodeRunner": ("cuda_graph", "CudaGraphDecodeRunner"),
     "load_spiderw": ("spiderw", "load_spiderw"),
     "write_spiderw": ("spiderw", "write_spiderw"),
+    "route_experts": ("routing", "route_experts"),
+    "quantize_fp8_blocks": ("fp8_blocks", "quantize_fp8_blocks"),
+    "fp8_block_matmul": ("fp8_blocks", "fp8_block_matmul"),
+    "fp8_block_linear": ("fp8_blocks", "fp8_block_linear"),
+    "fp8_expert_delta": ("fp8_blocks", "fp8_expert_delta"),
+    "Fp8BlockTensor": ("fp8_blocks", "Fp8BlockTensor"),
+    "Fp8BlockExperts": ("fp8_blocks", "Fp8BlockExperts"),
 }
 
 

@@ -22,6 +22,7 @@ from . import expert_parallel as ep_helpers
 from .config import from_any
 from .engine import BlockEngine
 from .dobu import ExpertChunkStore
+from .fp8_blocks import BLOCK, Fp8BlockExperts
 from .lumen import LumenWorkspace
 from .quant import Int4Tensor, quantize_fp8_per_channel, quantize_int4
 
@@ -67,6 +68,8 @@ class SpiderMoELayer(nn.Module):
         self._int4_w_down: Int4Tensor | None = None
         self._int4_w_gate: Int4Tensor | None = None
         self._fp8 = None
+        self._fp8_block_size = None                       # 128: experts in block-scaled fp8
+        self._fp8_experts: Fp8BlockExperts | None = None  # packed at the first forward
         self._engine: BlockEngine | None = None
         self._engine_key = None
 
@@ -91,12 +94,26 @@ class SpiderMoELayer(nn.Module):
         if hasattr(self, "expert_gates"):
             self._int4_w_gate = quantize_int4(torch.stack([g.weight.detach() for g in self.expert_gates]),
                                               group_size=group_size)
-        self._fp8 = None
+        self._fp8 = self._fp8_block_size = None
         self.invalidate()
 
     @torch.no_grad()
-    def quantize_experts_fp8(self) -> None:
-        """e4m3 expert weights with one fp32 scale per output channel (absmax/448)."""
+    def quantize_experts_fp8(self, block_size: int | None = None) -> None:
+        """e4m3 expert weights with one fp32 scale per output channel (absmax/448),
+        or, with block_size 128, per 128 x 128 block (``fp8_blocks``): the experts
+        then run on the fp8 tensor cores with their activations quantised too, one
+        scale per row and 128 columns.  The blocks are packed at the next forward
+        pass, on its device."""
+        if block_size is not None:
+            if block_size != BLOCK:
+                raise ValueError(f"block_size must be None (per output channel) or {BLOCK}, got {block_size}")
+            if self.offload_experts:
+                raise ValueError("block-scaled experts are resident: not with offload_experts")
+            self._int4_w_up = self._int4_w_down = self._int4_w_gate = self._fp8 = None
+            self._fp8_block_size = block_size
+            self.invalidate()
+            return
+        self._fp8_block_size = None
         stack = lambda j: torch.stack([ex[j].weight.detach() for ex in self.experts], dim=0)  # noqa: E731
         up = quantize_fp8_per_channel(stack(0))
         down = quantize_fp8_per_channel(stack(2))
@@ -110,13 +127,14 @@ class SpiderMoELayer(nn.Module):
     def dequantize_experts(self) -> None:
         """Clear quantised expert buffers and use the nn.Linear weights again."""
         self._int4_w_up = self._int4_w_down = self._int4_w_gate = None
-        self._fp8 = None
+        self._fp8 = self._fp8_block_size = None
         self.invalidate()
 
     def invalidate(self) -> None:
         """Drop packed device weights (call after changing parameters in place)."""
         self._engine = None
         self._engine_key = None
+        self._fp8_experts = None
 
     def _load_from_state_dict(self, *args, **kwargs):
         self.invalidate()
@@ -131,7 +149,7 @@ class SpiderMoELayer(nn.Module):
                 if self._int4_w_gate is not None:
                     int4["gate"] = self._int4_w_gate
             state = self.state_dict()
-            if self.offload_experts:  # dense parts only: the experts come from the store
+            if self._split_experts():  # dense parts only: the experts come from the store or the blocks
                 state = {k: v for k, v in state.items() if not k.startswith(("experts.", "expert_gates."))}
                 int4 = None
             self._engine = BlockEngine(self.cfg, state, device, act_dtype=act_dtype,
@@ -139,6 +157,22 @@ class SpiderMoELayer(nn.Module):
                                        int4=int4, fp8=self._fp8)
             self._engine_key = key
         return self._engine
+
+    def _split_experts(self) -> bool:
+        """Whether the experts run outside the block kernels (offloaded, or in block-scaled fp8)."""
+        return self.offload_experts or self._fp8_block_size is not None
+
+    @torch.no_grad()
+    def fp8_block_experts(self, device) -> Fp8BlockExperts:
+        device = torch.device(device)
+        if self._fp8_experts is None or self._fp8_experts.device != device:
+            stack = lambda ms, j, f: torch.stack([getattr(m if j is None else m[j], f).detach() for m in ms]).to(device)  # noqa: E731
+            gates = getattr(self, "expert_gates", None)
+            w = lambda ms, j: stack(ms, j, "weight").float()  # noqa: E731
+            self._fp8_experts = Fp8BlockExperts(
+                w(self.experts, 0), stack(self.experts, 0, "bias"), w(self.experts, 2), stack(self.experts, 2, "bias"),
+                w(gates, None) if gates is not None else None, stack(gates, None, "bias") if gates is not None else None)
+        return self._fp8_experts
 
     # ------------------------------------------------------------------ forward
     def forward(self, h, x0, loop_idx, return_stats=False):
@@ -150,6 +184,8 @@ class SpiderMoELayer(nn.Module):
         use_ep = self.expert_parallel and ep_helpers.ep_enabled()
         if self.offload_experts:
             out, taps = self._forward_offload(eng, h, x0, loop_idx)
+        elif self._fp8_block_size is not None:
+            out, taps = self._forward_fp8_blocks(eng, h, x0, loop_idx, use_ep)
         elif not use_ep and not return_stats:
             out = eng.forward(h, x0, loop_idx, loop_idx + 1).to(h.dtype)
             return self.lumen(out) if self.lumen is not None else out
@@ -191,6 +227,21 @@ class SpiderMoELayer(nn.Module):
         out = eng.epilogue(delta, inv, h, x0).to(h.dtype)
         return out, {"top_idx": top_idx, "top_w": top_w}
 
+    def _forward_fp8_blocks(self, eng, h, x0, loop_idx, use_ep):
+        """The block with block-scaled fp8 experts: routing and messages
+        (sb_block_route), the experts (sb_fp8_expert_delta; under expert
+        parallelism this rank's, summed across ranks), the LayerNorm epilogue
+        (sb_combine_ln).  Returns (out, routing taps)."""
+        rank, world = ep_helpers.get_rank_world() if use_ep else (0, 1)
+        n = h.numel() // h.shape[-1]
+        msgs, top_idx, top_w = eng.route(h, loop_idx)
+        delta = self.fp8_block_experts(h.device).delta(msgs, top_idx, top_w, rank, world, torch.float32)
+        if use_ep:
+            ep_helpers.all_reduce_sum_(delta)
+        inv = torch.arange(n, dtype=torch.int32, device=h.device).view(n, 1)
+        out = eng.epilogue(delta, inv, h, x0).to(h.dtype)
+        return out, {"top_idx": top_idx, "top_w": top_w}
+
     def _forward_ep(self, eng, h, x0, loop_idx):
         """Reference expert-parallel semantics (sparse_experts.py:38-43,66-67):
         every rank routes all tokens and computes their messages
@@ -210,7 +261,7 @@ class SpiderMoELayer(nn.Module):
         """All loops [loop_begin, loop_end) in one library call (model.py:445-448)."""
         n = h.numel() // h.shape[-1]
         eng = self.engine(h.device, h.dtype, n)
-        if self.offload_experts:  # the store's residency decisions run per loop on the host
+        if self._split_experts():  # loop by loop (the store's residency decisions run on the host)
             for loop_idx in range(loop_begin, self.cfg.num_loops if loop_end is None else loop_end):
                 h = self(h, x0, loop_idx)
             return h
@@ -235,7 +286,7 @@ class SpiderMoELayer(nn.Module):
         if self.lumen is not None:
             def loop_fn(hc, xc, loop_idx, out):
                 out.copy_(self.lumen(eng.forward(hc, xc, loop_idx, loop_idx + 1)).reshape(out.shape))
-        if (self.expert_parallel and ep_helpers.ep_enabled()) or self.offload_experts:
+        if (self.expert_parallel and ep_helpers.ep_enabled()) or self._split_experts():
             # the module's own loop (Lumen included); under expert parallelism
             # every rank holds the same rows, so the active sets agree and each
             # loop's all-reduce has the same shape everywhere

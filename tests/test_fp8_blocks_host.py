@@ -156,3 +156,13 @@ def test_c_abi_refuses_before_any_launch():
         x, 0, 32, 4, 8, 32, w, 0, 32, dy, dr, 1, p, p, None, p, n, None)
     assert back(x=None) == back(w=None) == back(dy=None) == back(dr=-1) == L.SB_ERR_ARG
     assert back(n=64) == L.SB_ERR_WORKSPACE
+
+
+def test_layer_refuses_other_block_sizes():
+    from spider_web_moe_b200 import ModelConfig, SpiderMoELayer
+
+    kw = dict(hidden_size=64, num_heads=4, num_experts=4, top_k=2, edges_per_expert=2, num_loops=2, expert_ffn_size=128)
+    with pytest.raises(ValueError):
+        SpiderMoELayer(ModelConfig(**kw)).quantize_experts_fp8(block_size=64)
+    with pytest.raises(ValueError):
+        SpiderMoELayer(ModelConfig(**kw, offload_experts=True)).quantize_experts_fp8(block_size=128)
