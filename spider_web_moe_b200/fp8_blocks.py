@@ -68,9 +68,13 @@ def check_status(device) -> None:
         raise L.SpiderB200Error(L.SB_ERR_DEVICE_STATUS, f"fp8_blocks: device status 0x{word:x}")
 
 
+_CHECK = bool(os.environ.get("SPIDER_B200_CHECK"))  # read once: the lookup costs a launch's share of host time
+
+
 def _finish(rc: int, where: str, device) -> None:
-    L.check(rc, where)
-    if os.environ.get("SPIDER_B200_CHECK"):
+    if rc != L.SB_OK:
+        L.check(rc, where)
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
         check_status(device)
 
 
@@ -364,17 +368,19 @@ class Fp8BlockExperts:
         out_dtype = messages.dtype if out_dtype is None else out_dtype
         n, k = top_indices.shape
         x = _unit_cols(messages)
-        idx = top_indices
+        idx, w = top_indices, top_weights
         if world > 1:
             idx = torch.where(idx % world == rank, idx, -1)
-        idx = idx.to(torch.int32).contiguous()
-        w = top_weights.to(torch.float32).contiguous()
+        if idx.dtype != torch.int32 or not idx.is_contiguous():
+            idx = idx.to(torch.int32).contiguous()
+        if w.dtype != torch.float32 or not w.is_contiguous():
+            w = w.to(torch.float32).contiguous()
         cols = -(-self.hidden // 4) * 4
-        out = torch.empty((n, cols), dtype=out_dtype, device=dev)
+        out = x.new_empty((n, cols), dtype=out_dtype)
         nbytes = lib.sb_fp8_expert_delta_workspace_bytes(self._ref, n, k)
         if nbytes == 0:
             raise L.SpiderB200Error(L.SB_ERR_ARG, "sb_fp8_expert_delta_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = x.new_empty((nbytes,), dtype=torch.uint8)
         rc = L.on_device(dev, lib.sb_fp8_expert_delta, self._ref, x.data_ptr(), code, max(x.stride(0), self.hidden),
                          idx.data_ptr(), w.data_ptr(), n, k, out.data_ptr(), _DTYPES[out_dtype], _status_ptr(dev),
                          ws.data_ptr(), nbytes)
@@ -389,22 +395,25 @@ def fp8_expert_delta(messages, top_indices, top_weights, experts: Fp8BlockExpert
     the messages' dtype.  Repeated ids of a token add their weights, weights <= 0
     and ids outside [0, E) are skipped; under expert parallelism each rank runs
     its own experts and the delta is summed across ranks.  Inference only."""
-    _need_cuda(messages, "fp8_expert_delta")
-    if messages.shape[-1] != experts.hidden or top_indices.shape != top_weights.shape or \
-            top_indices.shape[:-1] != messages.shape[:-1]:
-        raise ValueError(f"need messages [..., {experts.hidden}] and top_indices / top_weights [..., K], got "
-                         f"{tuple(messages.shape)}, {tuple(top_indices.shape)}, {tuple(top_weights.shape)}")
-    if not 1 <= top_indices.shape[-1] <= 64:
+    ms, ks, hidden = messages.shape, top_indices.shape, experts.hidden
+    if not ms or ms[-1] != hidden or ks != top_weights.shape or ks[:-1] != ms[:-1]:
+        raise ValueError(f"need messages [..., {hidden}] and top_indices / top_weights [..., K], got {tuple(ms)}, "
+                         f"{tuple(ks)}, {tuple(top_weights.shape)}")
+    k = ks[-1]
+    if not 1 <= k <= 64:
         raise ValueError("between 1 and 64 experts per token")
-    if any(t.device != experts.device for t in (messages, top_indices, top_weights)):
+    dev = experts.device
+    if messages.device != dev or top_indices.device != dev or top_weights.device != dev:
         raise ValueError("messages, routing and experts must be on one device")
     if torch.is_grad_enabled() and (messages.requires_grad or top_weights.requires_grad):
         raise NotImplementedError("fp8_expert_delta has no backward pass: call it under torch.no_grad()")
-    k = top_indices.shape[-1]
     use_ep = expert_parallel and ep_enabled()
     rank, world = get_rank_world() if use_ep else (0, 1)
-    delta = experts.delta(messages.reshape(-1, experts.hidden), top_indices.reshape(-1, k), top_weights.reshape(-1, k),
-                          rank, world, torch.float32 if use_ep else messages.dtype)
+    flat = len(ms) == 2
+    if not flat:
+        messages, top_indices = messages.reshape(-1, hidden), top_indices.reshape(-1, k)
+        top_weights = top_weights.reshape(-1, k)
+    delta = experts.delta(messages, top_indices, top_weights, rank, world, torch.float32 if use_ep else messages.dtype)
     if use_ep:
         delta = all_reduce_sum_(delta.contiguous()).to(messages.dtype)
-    return delta.reshape(messages.shape)
+    return delta if flat else delta.reshape(ms)
