@@ -540,11 +540,14 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * NC;
     uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + C::kOffMax);
     const uint32_t released_lead = kPair && rank != 0 ? mapa_shared(smem_u32(released), 0) : 0;
-    Ring<S> st;
-    Ring<4> rel;
-    int item = 0;
+    // One counter of blocks for the rings of stages, accumulators and scales, and
+    // one of items: beside 192 registers of sums and columns there is little room.
+    static_assert(S == 4 && C::kItemSlots == 8, "ring positions are bits of the counters");
+    uint32_t it = 0;
+    const int items = (total - first + stride - 1) / stride;
     bool ok = true;
-    for (int t = first; t < total && ok; t += stride, item = (item + 1) % C::kItemSlots) {
+    for (int item = 0; item < items && ok; ++item) {
+      const int t = first + item * stride;
       bool warp_live, second;
       {
         const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t, rank);
@@ -557,15 +560,15 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
-      for (int kk = 0; kk < nk; ++kk, st.next(), rel.next()) {
-        const int buf = rel.slot & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(&done[st.slot], st.parity, p.status, SB_DEVERR_EPI_WAIT))) {
+      for (int kk = 0; kk < nk; ++kk, ++it) {
+        const uint32_t slot = it & 3;
+        if (!__all_sync(0xffffffffu, mbar_wait(&done[slot], (it >> 2) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t t0 = lane_addr + buf * C::kAccCols;
-        const float* f = reinterpret_cast<const float*>(smem + C::kOffScale) + rel.slot * C::kScaleFloats;
+        const uint32_t t0 = lane_addr + (it & 1) * C::kAccCols;
+        const float* f = reinterpret_cast<const float*>(smem + C::kOffScale) + slot * C::kScaleFloats;
         const uint64_t s0 = pair_of(f[r]), s1 = kBRows ? s0 : pair_of(f[C::kBM + r]);
         // columns 32 j .. of the warp's 2 x 64: two loads in flight, the second
         // pair over the first pair's additions
@@ -587,8 +590,8 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&released[rel.slot]);
-            if (kPair && rank != 0) mbar_arrive_leader(released_lead + 8u * rel.slot);
+            mbar_arrive(&released[slot]);
+            if (kPair && rank != 0) mbar_arrive_leader(released_lead + 8u * slot);
           }
         };
         if (warp_live && kBRows) {
@@ -631,12 +634,12 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
       }
       // the item again, so that its fields need no registers beside the sums
-      int t_again = t;
+      int t_again = first + item * stride;
       asm volatile("" : "+r"(t_again));
       const F8Item w = f8_item<kPair>(prefix, s_off, G, n_tiles, kTileCols, p.max_rows, t_again, rank);
       const bool live = r < w.rows;
       const int64_t row = w.row0 + r;
-      const float* s_bias = reinterpret_cast<const float*>(smem + C::kOffItem) + item * C::kItemFloats + part * NC;
+      const float* s_bias = reinterpret_cast<const float*>(smem + C::kOffItem) + (item & 7) * C::kItemFloats + part * NC;
       float acc[2][NC];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
