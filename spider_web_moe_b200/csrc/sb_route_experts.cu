@@ -157,17 +157,28 @@ SB_DEVINL int take_top(const uint32_t (&key)[V], uint32_t* list, uint32_t* taken
   const uint32_t me = 1u << lane;
   const uint32_t last_id = static_cast<uint32_t>(lane * V) + kPlaceMask<V>;
   int at = 0;
+  const uint32_t list_addr = smem_u32(mylist);
+  const uint32_t taken_addr = smem_u32(taken);
   for (int j = 0; j < K; ++j) {
     const uint32_t h = head & ~kPlaceMask<V>;
     const uint32_t top = __reduce_max_sync(0xffffffffu, h);
     const uint32_t who = __ballot_sync(0xffffffffu, h == top);
-    if ((who & (0u - who)) == me) {  // the lowest lane of them
-      *reinterpret_cast<uint2*>(taken + 2 * j) = make_uint2(last_id - (head & kPlaceMask<V>), h);
-      ++at;
-      head = V > 1 && at < V ? mylist[at] : 0;
-    }
-    __syncwarp();
+    // the lowest lane of them writes its expert and moves on: predicated, so that
+    // the round has no branch to reconverge from
+    const uint32_t id = last_id - (head & kPlaceMask<V>);
+    asm volatile(
+        "{\n\t.reg .pred w, m;\n\t"
+        "setp.eq.u32 w, %2, %3;\n\t"
+        "@w st.shared.v2.b32 [%4], {%5, %6};\n\t"
+        "@w add.s32 %0, %0, 1;\n\t"
+        "setp.lt.and.s32 m, %0, %8, w;\n\t"
+        "@w mov.b32 %1, 0;\n\t"
+        "@m ld.shared.b32 %1, [%7];\n\t}"
+        : "+r"(at), "+r"(head)
+        : "r"(who & (0u - who)), "r"(me), "r"(taken_addr + 8 * j), "r"(id), "r"(h), "r"(list_addr + 4 * (at + 1)), "n"(V)
+        : "memory");
   }
+  __syncwarp();
   *head_out = head;
   *used = at;
   const uint2 t = lane < K ? *reinterpret_cast<const uint2*>(taken + 2 * lane) : make_uint2(0, 0);
@@ -436,8 +447,10 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
 }
 
 // Gradient of the weights with respect to the logits, the selection held fixed:
-//   ds_j = scale (g_j - (sum_k g_k s_k) / D) / D   (renormalised, D = sum s)
+//   ds_j = scale (sum_k s_k (g_j - g_k) / D) / D   (renormalised, D = sum s)
 //   ds_j = scale g_j / D'                          (D' = 1, or the floor 1e-9)
+// The sum of differences does not cancel: it is exactly 0 where all g are equal,
+// a single expert's among them.
 //   softmax: dl_i = s_i (ds_i - sum_k ds_k s_k);  sigmoid: dl_j = ds_j s_j (1 - s_j)
 template <typename T, int V, bool kVec>
 __global__ void __launch_bounds__(256)
@@ -481,14 +494,18 @@ route_experts_backward_kernel(const T* __restrict__ logits, const __grid_constan
   if (p.renorm) {
     const float sum = warp_sum(sw);
     const float d = sum < 1e-9f ? 1e-9f : sum;
-    const float dot = warp_sum(g * sw);
-    ds = p.scale * (sum < 1e-9f ? g : g - dot / d) / d;
+    float diff = 0.f;
+    for (int j = 0; j < p.K; ++j)
+      diff = fmaf(__shfl_sync(0xffffffffu, sw, j), g - __shfl_sync(0xffffffffu, g, j), diff);
+    ds = p.scale * (sum < 1e-9f ? g : diff / d) / d;
   }
   if (masked) ds = 0.f;
   float dv[V];
   float add;
   if (p.score == SB_SCORE_SOFTMAX) {
-    const float dot = warp_sum(ds * ssel);
+    // (renormalised, sum_k ds_k s_k is 0: only rounding would be left of it)
+    const bool zero = p.renorm && warp_sum(sw) >= 1e-9f;
+    const float dot = zero ? 0.f : warp_sum(ds * ssel);
 #pragma unroll
     for (int v = 0; v < V; ++v) dv[v] = -dot;
     add = ds;

@@ -201,6 +201,18 @@ def test_gradient_against_differences(cuda_device):
         assert (leaf.grad.cpu().double() - num).abs().max() < 1e-5
 
 
+def test_equal_upstream_gradients_cancel_exactly(cuda_device):
+    """Renormalised weights sum to a constant: with the same upstream gradient for
+    all of a token's weights (a single expert's among them) the gradient is 0."""
+    x = torch.randn(50, 40, device=cuda_device)
+    for score in ("softmax", "sigmoid"):
+        for k in (1, 5):
+            leaf = x.clone().requires_grad_()
+            _, w = route_experts(leaf, k, score=score)
+            w.backward(torch.randn(50, 1, device=cuda_device).expand(50, k))
+            assert (leaf.grad == 0).all()
+
+
 def test_masked_rows_have_zero_gradient(cuda_device):
     rows = torch.randn(3, 8)
     rows[0] = float("-inf")
