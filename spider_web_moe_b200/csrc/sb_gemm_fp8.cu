@@ -1304,14 +1304,18 @@ static int launch_f8_decode(const sb_fp8_matmul_args& a, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, mx, mw, mg, a, splits));
 }
 
-// Rows per group (of a plain product: rows) up to which the weights-as-M
-// schedule runs, and its column count.
+// Column count of the weights-as-M schedule, or 0 for the row-tile schedules.
+// Plain products: up to 64 rows it is bound by the weights' bytes.  Beyond, while
+// its items of 128 x 64 fit the GPU at once: a block of k takes it about 0.45 us
+// and a 256 x 256 pair tile 0.65 us, and the same outputs are eight times the
+// items, which can then split k as well (128 x 2048 x 4096: 17.5 us in row tiles,
+// 11.8 us so).  Grouped products: by the average rows of a group.
 static int decode_columns(const sb_fp8_matmul_args& a) {
   if (a.b_block_rows != 128) return 0;
   if (!a.offsets) {
     if (a.max_rows <= 32) return a.max_rows <= 16 ? 16 : 32;
-    // up to 128 rows, in tiles of 64, while their items do not fill the GPU
-    return a.max_rows <= 64 || (a.max_rows <= 128 && (a.n + 127) / 128 * 2 <= current_sm_count()) ? 64 : 0;
+    const int64_t items = static_cast<int64_t>((a.max_rows + 63) / 64) * ((a.n + 127) / 128);
+    return a.max_rows <= 64 || items <= current_sm_count() ? 64 : 0;
   }
   const int per_group = a.max_rows / a.num_groups;
   return per_group <= 4 ? 16 : (per_group <= 20 ? 32 : (per_group <= 48 ? 64 : 0));
