@@ -318,8 +318,8 @@ SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t ldx, int m, 
  *   delta[t] = sum over t's experts of w * (down(q(act(up(q(messages[t]))))) + b_down)
  * in slot order.  messages: row pitch ld elements.  delta: [n_tokens, hidden
  * rounded up to a multiple of 4] fp32 or bf16 (the extra columns hold no
- * values).  top_k <= 64.  Workspace status word at offset 0 unless `status` is
- * given; the workspace needs no initial contents otherwise. */
+ * values).  num_experts <= 256, top_k <= 64.  Workspace status word at offset 0
+ * unless `status` is given; the workspace needs no initial contents otherwise. */
 typedef struct sb_fp8_experts {
   int num_experts, hidden, ffn;
   int activation; /* SB_ACT_GELU / SB_ACT_SWIGLU */

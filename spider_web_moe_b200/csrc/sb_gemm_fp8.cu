@@ -1501,8 +1501,10 @@ struct F8DeltaBuffers {
   int* status;
 };
 
+constexpr int kF8MaxExperts = 256;  // as many as sb_group takes
+
 static bool f8_experts_ok(const sb_fp8_experts* x) {
-  return x && x->num_experts >= 1 && x->num_experts <= kF8MaxG && x->hidden >= 1 && x->ffn >= 1 &&
+  return x && x->num_experts >= 1 && x->num_experts <= kF8MaxExperts && x->hidden >= 1 && x->ffn >= 1 &&
          (x->activation == SB_ACT_GELU || x->activation == SB_ACT_SWIGLU) && x->ld_in % 16 == 0 && x->ld_in >= x->hidden &&
          x->ld_ffn % 16 == 0 && x->ld_ffn >= x->ffn;
 }

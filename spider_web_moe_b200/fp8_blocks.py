@@ -335,8 +335,8 @@ class Fp8BlockExperts:
             raise ValueError("expert weights must be w_up / w_gate [E, U, H] and w_down [E, H, U]")
         if any(w is not None and w.q.device != self.device for w in (self.w_down, self.w_gate)):
             raise ValueError("all expert weights must be on one device")
-        if self.num_experts < 1 or self.ffn < 1 or self.hidden < 1 or self.num_experts > 1024:
-            raise ValueError("between 1 and 1024 experts of at least one row and column")
+        if self.num_experts < 1 or self.ffn < 1 or self.hidden < 1 or self.num_experts > 256:
+            raise ValueError("between 1 and 256 experts of at least one row and column")
         if self.w_gate is None and b_gate is not None:
             raise ValueError("b_gate needs w_gate")
         if self.w_gate is not None and self.w_gate.pitch != self.w_up.pitch:

@@ -117,6 +117,36 @@ def test_product(m, k, n, br, cuda_device):
     check_status(cuda_device)
 
 
+# more 128 x 64 items than SMs: tiles of 128 rows (up to 128 rows) and of CTA pairs
+TILES = [(100, 160, 9700), (33 + 64, 2048, 9601), (257, 200, 4000), (700, 130, 2056), (513, 1040, 3900), (1029, 16, 1300)]
+
+
+@pytest.mark.parametrize("m,k,n", TILES)
+@pytest.mark.parametrize("br", [128, 1])
+def test_product_row_tiles(m, k, n, br, cuda_device):
+    a = quantize_fp8_blocks(rand(m, k, seed=m).to(cuda_device))
+    b = quantize_fp8_blocks(rand(n, k, seed=n + 1).to(cuda_device), br)
+    ad, bd = a.dequantize().double().cpu(), b.dequantize().double().cpu()
+    for dtype in (torch.float32, torch.bfloat16):
+        got = fp8_block_matmul(a, b, dtype)
+        check(got, ad, bd, f"{dtype}")
+        for off in (11, 16):  # an output that bulk stores cannot address, and one that they can
+            big = torch.full((m + 9, n + 40), 7.0, device=cuda_device, dtype=dtype)
+            fp8_block_matmul(a, b, out=big[5:m + 5, off:n + off])
+            assert torch.equal(big[5:m + 5, off:n + off], got)
+            big[5:m + 5, off:n + off] = 7
+            assert (big == 7).all()
+    check_status(cuda_device)
+
+
+def test_product_long_k_and_one_row(cuda_device):
+    """128 blocks of k split over a cluster, and one block in a problem that could be split."""
+    for m, k, n in ((1, 16384, 256), (1, 128, 128), (3, 40000, 130), (16, 17000, 1)):
+        a = quantize_fp8_blocks(rand(m, k, seed=m).to(cuda_device))
+        b = quantize_fp8_blocks(rand(n, k, seed=n + 1).to(cuda_device), 128)
+        check(fp8_block_matmul(a, b, torch.float32), a.dequantize().double().cpu(), b.dequantize().double().cpu())
+
+
 def test_product_rows_do_not_mix(cuda_device):
     """A NaN row and rows of very different size leave the others as they were."""
     x = rand(140, 256, seed=8)
@@ -186,7 +216,8 @@ def grouped(epi, e, u, h, counts, seed, device):
 
 
 GROUPS = [(1, 128, 128, [3]), (3, 129, 70, [0, 1, 200]), (5, 256, 384, [130, 0, 32, 33, 64]),
-          (40, 64, 256, [i % 4 for i in range(40)]), (4, 300, 512, [0, 0, 0, 0]), (2, 1000, 1040, [257, 128])]
+          (40, 64, 256, [i % 4 for i in range(40)]), (4, 200, 300, [70, 0, 33, 17]),
+          (6, 300, 256, [129, 300, 128, 0, 256, 31]), (4, 300, 512, [0, 0, 0, 0]), (2, 1000, 1040, [257, 128])]
 
 
 @pytest.mark.parametrize("e,u,h,counts", GROUPS)
@@ -402,6 +433,37 @@ def test_expert_delta_routing_rules(cuda_device):
     parts = sum(ex.delta(x.to(cuda_device), idx.to(cuda_device), w.to(cuda_device), r, 3, torch.float32) for r in range(3))
     torch.testing.assert_close(parts.double().cpu(), ex.delta(x.to(cuda_device), idx.to(cuda_device), w.to(cuda_device),
                                                               out_dtype=torch.float32).double().cpu(), rtol=2.0 ** -20, atol=1e-6)
+
+
+def test_many_experts(cuda_device):
+    """256 experts (the limit), most without a token; one more is refused."""
+    g = torch.Generator().manual_seed(3)
+    w = torch.randint(0, 120, (256, 32, 16), generator=g).to(torch.uint8).to(cuda_device).view(torch.float8_e4m3fn)
+    up = Fp8BlockTensor(w, torch.full((256, 1, 1), 2.0 ** -6, device=cuda_device), 128)
+    down = Fp8BlockTensor(w.view(torch.uint8).view(256, 16, 32).view(torch.float8_e4m3fn),
+                          torch.full((256, 1, 1), 2.0 ** -6, device=cuda_device), 128)
+    ex = Fp8BlockExperts(up, None, down, None)
+    x = rand(20, 16, seed=4)
+    idx = torch.randint(0, 256, (20, 3), generator=g)
+    idx[0] = torch.tensor([0, 255, 128])
+    wt = torch.rand(20, 3, generator=g) + 0.1
+    got = fp8_expert_delta(x.to(cuda_device), idx.to(cuda_device), wt.to(cuda_device), ex)
+    want, _ = delta_oracle(ex, dict(up=None, down=None), x, idx, wt)
+    assert ((got.double().cpu() - want).norm(dim=1) / want.norm(dim=1)).max() < 2.0 ** -5
+    with pytest.raises(ValueError):
+        big = lambda t: Fp8BlockTensor(torch.cat([t.q.view(torch.uint8), t.q[:1].view(torch.uint8)]).view(t.q.dtype),  # noqa: E731
+                                       torch.ones(257, 1, 1, device=cuda_device), 128)
+        Fp8BlockExperts(big(up), None, big(down), None)
+
+
+def test_all_routes_dropped(cuda_device):
+    """No token keeps an expert: zeros, from kernels without an item."""
+    ex, _ = make_experts(6, 64, 48, True, 7, cuda_device)
+    for n in (1, 700):
+        x = rand(n, 64, seed=8).to(cuda_device)
+        idx = torch.full((n, 2), -1, device=cuda_device)
+        assert (fp8_expert_delta(x, idx, torch.ones(n, 2, device=cuda_device), ex) == 0).all()
+    check_status(cuda_device)
 
 
 def test_two_graphs_and_a_stream(cuda_device):
