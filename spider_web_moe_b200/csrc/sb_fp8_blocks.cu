@@ -277,8 +277,11 @@ __global__ void __launch_bounds__(256, 4) fp8_quantize_block_bf16_kernel(const s
 // bf16 matrices whose rows are contiguous (transposed views), rows a multiple of 8
 // and columns on 16-byte boundaries: the tile lies in shared memory as [col][row]
 // and a thread takes two neighbouring rows, one 32-bit word per column, and a
-// quarter of the columns.
-__global__ void __launch_bounds__(256, 4) fp8_quantize_transposed_bf16_kernel(const sb_fp8_quantize_args p) {
+// quarter of the columns.  kBoth: the matrix itself (d: 1 x 128 blocks of p's
+// transpose) is quantised from the same loads, before they go to shared memory.
+template <bool kBoth>
+__global__ void __launch_bounds__(256, 4)
+fp8_quantize_transposed_bf16_kernel(const sb_fp8_quantize_args p, const sb_fp8_quantize_args d) {
   constexpr int kPitch = 136;  // elements; 68 words, so a warp's 32 row pairs meet no bank conflict
   __shared__ __align__(16) __nv_bfloat16 tile[128 * kPitch];
   __shared__ uint32_t s_max[256];
@@ -300,6 +303,32 @@ __global__ void __launch_bounds__(256, 4) fp8_quantize_transposed_bf16_kernel(co
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(tile + (i * 16 + (tid >> 4)) * kPitch + r) = v[i];
+    if constexpr (kBoth) {
+      // 16 lanes hold a block of the untransposed matrix; two of them share a
+      // register in the shuffles
+      constexpr uint32_t kAbs = 0x7fff7fffu;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        uint32_t m[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint4 u = v[i + k];
+          m[k] = __vmaxu2(__vmaxu2(u.x & kAbs, u.y & kAbs), __vmaxu2(u.z & kAbs, u.w & kAbs));
+        }
+        uint32_t w = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) w = __vmaxu2(w, __shfl_xor_sync(0xffffffffu, w, o));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = (i + k) * 16 + (tid >> 4);
+          if (c >= nc || r >= nr) continue;
+          const Fp8Scale s = fp8_scale(k ? w & 0xffff0000u : w << 16);
+          if ((tid & 15) == 0) d.scale[(c0 + c) * d.scale_row + blockIdx.y * d.scale_col] = s.scale;
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(d.q) + (c0 + c) * d.ldq + r0 + r) =
+              make_uint2(fp8_pack4_bf16(v[i + k].x, v[i + k].y, s.inv), fp8_pack4_bf16(v[i + k].z, v[i + k].w, s.inv));
+        }
+      }
+    }
   }
   __syncthreads();
   const int pair = tid & 63, quarter = tid >> 6;
@@ -392,13 +421,21 @@ static int quantize_typed(const sb_fp8_quantize_args& p, cudaStream_t st) {
   if (p.rows > 65535 * 128) return SB_ERR_UNSUPPORTED;  // a grid's y extent
   const dim3 tiles((p.cols + 127) / 128, (p.rows + 127) / 128, p.batch);
   if (sizeof(T) == 2 && p.x_row == 1 && p.x_col != 1 && base && p.x_col % 8 == 0 && p.rows % 8 == 0)
-    return launch(fp8_quantize_transposed_bf16_kernel, tiles, dim3(256), 0, st, p);
+    return launch(fp8_quantize_transposed_bf16_kernel<false>, tiles, dim3(256), 0, st, p, p);
   if (sizeof(T) == 2 && p.x_col == 1 && base && p.x_row % 8 == 0 && p.cols % 8 == 0)
     return launch(fp8_quantize_block_bf16_kernel, tiles, dim3(256), 0, st, p);
   if (p.x_row == 1 && p.x_col != 1)
     return base && p.x_col % kAlign == 0 ? launch_tile<T, true, true>(p, st) : launch_tile<T, true, false>(p, st);
   return p.x_col == 1 && base && p.x_row % kAlign == 0 ? launch_tile<T, false, true>(p, st)
                                                        : launch_tile<T, false, false>(p, st);
+}
+
+int fp8_quantize_both(const sb_fp8_quantize_args& d, const sb_fp8_quantize_args& t, cudaStream_t st) {
+  if (d.dtype != SB_BF16 || d.block_rows != 1 || d.batch != 1 || d.row_index || d.x_col != 1 || d.x_row % 8 ||
+      d.cols % 8 || reinterpret_cast<uintptr_t>(d.x) % 16 || d.cols > 65535 * 128 || d.rows <= 0)
+    return SB_ERR_UNSUPPORTED;
+  return launch(fp8_quantize_transposed_bf16_kernel<true>, dim3((t.cols + 127) / 128, (t.rows + 127) / 128), dim3(256), 0,
+                st, t, d);
 }
 
 }  // namespace sb

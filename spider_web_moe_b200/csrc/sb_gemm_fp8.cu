@@ -1392,12 +1392,17 @@ static F8Buf f8_buf(Carver& c, int rows, int cols, int block_rows) {
   }
   return b;
 }
-static int f8_quantize(const F8Buf& b, const void* x, int dtype, int rows, int cols, int64_t x_row, int64_t x_col,
-                       int block_rows, void* stream) {
+static sb_fp8_quantize_args f8_quantize_args(const F8Buf& b, const void* x, int dtype, int rows, int cols, int64_t x_row,
+                                             int64_t x_col, int block_rows) {
   sb_fp8_quantize_args q = {};
   q.x = x; q.dtype = dtype; q.block_rows = block_rows; q.batch = 1; q.rows = rows; q.cols = cols;
   q.x_row = x_row; q.x_col = x_col; q.q = b.q; q.ldq = b.ld;
   q.scale = b.s; q.scale_row = b.s_row; q.scale_col = b.s_col;
+  return q;
+}
+static int f8_quantize(const F8Buf& b, const void* x, int dtype, int rows, int cols, int64_t x_row, int64_t x_col,
+                       int block_rows, void* stream) {
+  const sb_fp8_quantize_args q = f8_quantize_args(b, x, dtype, rows, cols, x_row, x_col, block_rows);
   return sb_fp8_quantize_blocks(&q, stream);
 }
 static int f8_product(const F8Buf& a, const F8Buf& b, int b_block_rows, int m, int n, int k, void* out, int out_dtype,
@@ -1474,13 +1479,18 @@ extern "C" SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t l
   const F8Buf dq = f8_buf(c, m, n, 1), wt = f8_buf(c, k, n, 128), dt = f8_buf(c, n, m, 1), xt = f8_buf(c, k, m, 1);
   if (!workspace || c.overflow) return SB_ERR_WORKSPACE;
 #define SB_TRY(e) do { const int rc = (e); if (rc) return rc; } while (0)
+  // dy along its rows for dx and along its columns for dw, in one pass where it can
+  const bool both = dx && dw &&
+                    fp8_quantize_both(f8_quantize_args(dq, dy, dtype, m, n, dy_row, dy_col, 1),
+                                      f8_quantize_args(dt, dy, dtype, n, m, dy_col, dy_row, 1),
+                                      static_cast<cudaStream_t>(stream)) == SB_OK;
   if (dx) {  // the blocks of w^T are the transposed blocks of w: the forward pass's values
     SB_TRY(f8_quantize(wt, w, w_dtype, k, n, 1, ldw, 128, stream));
-    SB_TRY(f8_quantize(dq, dy, dtype, m, n, dy_row, dy_col, 1, stream));
+    if (!both) SB_TRY(f8_quantize(dq, dy, dtype, m, n, dy_row, dy_col, 1, stream));
     SB_TRY(f8_product(dq, wt, 128, m, k, n, dx, dtype, status, stream));
   }
   if (dw) {
-    SB_TRY(f8_quantize(dt, dy, dtype, n, m, dy_col, dy_row, 1, stream));
+    if (!both) SB_TRY(f8_quantize(dt, dy, dtype, n, m, dy_col, dy_row, 1, stream));
     SB_TRY(f8_quantize(xt, x, dtype, k, m, 1, ldx, 1, stream));
     SB_TRY(f8_product(dt, xt, 1, n, k, m, dw, w_dtype, status, stream));
   }

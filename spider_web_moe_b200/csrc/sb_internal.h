@@ -169,6 +169,11 @@ int select_dense(const float* logits, int64_t ld, int n_tokens, int E, int K, in
 int dequant_to_bf16(int wfmt, const void* q, const void* scales, int group_size, int64_t rows, int64_t k, void* out,
                     cudaStream_t st);
 
+// A bf16 matrix d (1 x 128 blocks, unit column stride, rows on 16-byte boundaries,
+// columns a multiple of 8) and its transpose t, both quantised from one pass over
+// it (sb_fp8_blocks.cu); SB_ERR_UNSUPPORTED for other matrices.
+int fp8_quantize_both(const sb_fp8_quantize_args& d, const sb_fp8_quantize_args& t, cudaStream_t st);
+
 // Device properties cached per device.
 int current_sm_count();
 int current_cc_major();

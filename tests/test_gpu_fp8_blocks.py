@@ -265,7 +265,8 @@ def test_grouped_product(epi, e, u, h, counts, cuda_device):
         assert (err <= 2.0 ** -4 * (y.abs() + slack) + 2.0 ** -10 * se + slack).all()
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 64, 48), (40, 300, 130), (257, 512, 384), (7, 1000, 2056), (130, 129, 1)])
+@pytest.mark.parametrize("m,k,n", [(1, 64, 48), (40, 300, 130), (257, 512, 384), (7, 1000, 2056), (130, 129, 1),
+                                   (300, 264, 136), (129, 72, 8)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_linear_and_gradients(m, k, n, dtype, cuda_device):
     x, w, dy = rand(m, k, seed=1, dtype=dtype), rand(n, k, seed=2, dtype=dtype), rand(m, n, seed=3, dtype=dtype)
