@@ -1064,6 +1064,11 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       const int feat = w.n0 + quarter * 32 + lane;
       const bool fvalid = feat < p.n;
       const bool warp_live = half * NC < w.rows;  // some token column of this warp is valid
+      // the item's operands first: their loads pass under the products
+      const float bias = p.bias && fvalid ? p.bias[w.g * p.bias_group + feat] : 0.f;
+      const float bgate = kGate && p.bias_gate && fvalid ? p.bias_gate[w.g * p.bias_group + feat] : 0.f;
+      const float row_scale = !kQuant && p.row_scale && lane < NC && half * NC + lane < w.rows
+                                  ? p.row_scale[w.row0 + half * NC + lane] : 1.f;
       uint64_t sum[NT][NC / 2];
 #pragma unroll
       for (int h = 0; h < NT; ++h)
@@ -1099,15 +1104,6 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < NC / 2; ++i)
           asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[h][2 * i]), "=f"(acc[h][2 * i + 1]) : "l"(sum[h][i]));
-      const float bias = p.bias && fvalid ? p.bias[w.g * p.bias_group + feat] : 0.f;
-      auto store_linear = [&](int col, float v) {
-        const int64_t row = w.row0 + col;
-        v += bias;
-        if (p.row_scale) v *= p.row_scale[row];
-        if (!fvalid) return;
-        if (p.out_dtype == SB_F32) static_cast<float*>(p.out)[row * p.ldo + feat] = v;
-        else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + feat] = __float2bfloat16_rn(v);
-      };
       if constexpr (!kQuant) {
         if (splits > 1) {
           // this CTA's partial sums; every CTA of the cluster then finishes kN /
@@ -1120,10 +1116,13 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
           if (half * NC + i >= w.rows) break;
-          store_linear(half * NC + i, acc[0][i]);
+          const int64_t row = w.row0 + half * NC + i;
+          const float v = (acc[0][i] + bias) * __shfl_sync(0xffffffffu, row_scale, i);
+          if (!fvalid) continue;
+          if (p.out_dtype == SB_F32) static_cast<float*>(p.out)[row * p.ldo + feat] = v;
+          else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + feat] = __float2bfloat16_rn(v);
         }
       } else {
-        const float bgate = kGate && p.bias_gate && fvalid ? p.bias_gate[w.g * p.bias_group + feat] : 0.f;
         float y[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
