@@ -18,10 +18,11 @@
 // 1 x 128 block is the four threads of one token row) need no pass over memory
 // of their own.
 //
-// Two schedules.  One CTA per tile of 128 rows (decode batches, small groups);
+// Three schedules.  One CTA per tile of 128 rows (small groups, quantised outputs);
 // CTA pairs for tiles of 256 rows (cta_group::2): each CTA loads its own 128
 // rows of a and half of the weight rows, which halves the weight traffic into
-// shared memory, the limit of the one-CTA tile.
+// shared memory, the limit of the one-CTA tile; and one with the roles swapped
+// for decode batches (second half of this file).
 //
 // Scales come through shared memory from a warp of their own, which works up to
 // four blocks ahead: it loads a block's scales, multiplies them, writes them to
@@ -288,6 +289,7 @@ __global__ void __launch_bounds__(F8Cfg<kPair>::kThreads, 1)
 f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs,
                const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmG,
                const __grid_constant__ CUtensorMap tmO, const sb_fp8_matmul_args p, const int tma_out) {
+  static_assert(!kPair || EPI == SB_EPI_LINEAR, "quantised outputs run one CTA per tile");
   using C = F8Cfg<kPair>;
   constexpr int S = C::kStages;
   constexpr bool kGate = EPI == SB_EPI_SWIGLU;
@@ -780,7 +782,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       }
     }
   }
-  if (kPair && !kQuant && warp < C::kEpiWarps && lane == 0) tma_store_wait_all();  // stores done before the CTA leaves
+  if (kPair && warp < C::kEpiWarps && lane == 0) tma_store_wait_all();  // stores done before the CTA leaves
   __syncwarp();
   tc_fence_before();
   if constexpr (kPair) cluster_sync();  // neither CTA leaves while the other may still signal it
@@ -1320,7 +1322,13 @@ static int decode_columns(const sb_fp8_matmul_args& a) {
   return per_group <= 4 ? 16 : (per_group <= 20 ? 32 : (per_group <= 48 ? 64 : 0));
 }
 
-// Pairs pay when the rows per group fill their 256-row tiles.
+// LINEAR products: pairs pay when the rows per group fill their 256-row tiles (the
+// down product of 64 experts x 256 rows, k 1024, n 2048: 72 us against 100; of
+// groups of 0 to 1900 rows 112 against 121).  A quantised epilogue is the tail of
+// each item and takes as long in both schedules, so there the halved weight traffic
+// buys nothing (up product, k 2048, 2 x 1024: 120 us both; 16 x 1024 rows, k 4096: 370
+// against 378) and the half-empty last tiles of the groups cost (uneven groups: 184
+// against 149): those products run one CTA per tile.
 static bool use_pair(const sb_fp8_matmul_args& a) { return a.max_rows / a.num_groups > 128; }
 
 }  // namespace sb
@@ -1357,12 +1365,12 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
     SB_F8_DECODE(SB_EPI_LINEAR);
   }
 #undef SB_F8_DECODE
+  if (a.epilogue == SB_EPI_SWIGLU) return launch_f8<SB_EPI_SWIGLU, false, false>(a, st);
+  if (a.epilogue == SB_EPI_GELU) return launch_f8<SB_EPI_GELU, false, false>(a, st);
   const bool pair = use_pair(a);
-#define SB_F8(EPI, ROWS) return pair ? launch_f8<EPI, ROWS, true>(a, st) : launch_f8<EPI, ROWS, false>(a, st)
-  if (a.epilogue == SB_EPI_SWIGLU) SB_F8(SB_EPI_SWIGLU, false);
-  if (a.epilogue == SB_EPI_GELU) SB_F8(SB_EPI_GELU, false);
-  if (a.b_block_rows == 1) SB_F8(SB_EPI_LINEAR, true);
-  SB_F8(SB_EPI_LINEAR, false);
+#define SB_F8(ROWS) return pair ? launch_f8<SB_EPI_LINEAR, ROWS, true>(a, st) : launch_f8<SB_EPI_LINEAR, ROWS, false>(a, st)
+  if (a.b_block_rows == 1) SB_F8(true);
+  SB_F8(false);
 #undef SB_F8
 }
 
