@@ -25,6 +25,7 @@ from .expert_parallel import all_reduce_sum_, ep_enabled, get_rank_world
 
 BLOCK = 128
 _DTYPES = {torch.float32: L.SB_F32, torch.bfloat16: L.SB_BF16}
+_ID_TYPES = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
 def _dtype_code(t: torch.Tensor, what: str) -> int:
@@ -290,7 +291,7 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
         raise ValueError("packed weights need 128 x 128 blocks")
     _need_cuda(x, "fp8_block_linear")
     flat = len(xs) == 2
-    x2 = x if flat else x.reshape(-1, ws[1])
+    x2 = x if flat else x.reshape(xs[:-1].numel(), ws[1])
     if torch.is_grad_enabled() and (x.requires_grad or (packed is None and w.requires_grad)):
         y = _Fp8Linear.apply(x2, None if packed is not None else w, packed)
     else:
@@ -369,10 +370,14 @@ class Fp8BlockExperts:
         n, k = top_indices.shape
         x = _unit_cols(messages)
         idx, w = top_indices, top_weights
+        if idx.dtype != torch.int32:
+            if idx.dtype == torch.int64:  # ids outside [0, E) stay outside
+                idx = idx.clamp(-1, self.num_experts)
+            idx = idx.to(torch.int32)
         if world > 1:
             idx = torch.where(idx % world == rank, idx, -1)
-        if idx.dtype != torch.int32 or not idx.is_contiguous():
-            idx = idx.to(torch.int32).contiguous()
+        if not idx.is_contiguous():
+            idx = idx.contiguous()
         if w.dtype != torch.float32 or not w.is_contiguous():
             w = w.to(torch.float32).contiguous()
         cols = -(-self.hidden // 4) * 4
@@ -402,6 +407,8 @@ def fp8_expert_delta(messages, top_indices, top_weights, experts: Fp8BlockExpert
     k = ks[-1]
     if not 1 <= k <= 64:
         raise ValueError("between 1 and 64 experts per token")
+    if top_indices.dtype not in _ID_TYPES:
+        raise TypeError(f"top_indices must be integers, got {top_indices.dtype}")
     dev = experts.device
     if messages.device != dev or top_indices.device != dev or top_weights.device != dev:
         raise ValueError("messages, routing and experts must be on one device")

@@ -528,3 +528,41 @@ def test_training_step_captured(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     fp8_block_linear(x, w).backward(dy)
     assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_expanded_gradient(dtype, cuda_device):
+    """A gradient of stride 0 in both dimensions gives what its dense copy gives."""
+    x = rand(37, 200, seed=1, dtype=dtype).to(cuda_device).requires_grad_()
+    w = rand(130, 200, seed=2, dtype=dtype).to(cuda_device).requires_grad_()
+    one = torch.ones(1, 1, dtype=dtype, device=cuda_device)
+    got = torch.autograd.grad(fp8_block_linear(x, w), (x, w), one.expand(37, 130))
+    want = torch.autograd.grad(fp8_block_linear(x, w), (x, w), one.repeat(37, 130))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_linear_without_columns(cuda_device):
+    """Leading dimensions and no elements to sum over: zeros."""
+    y = fp8_block_linear(torch.ones(2, 3, 0, device=cuda_device), torch.ones(5, 0, device=cuda_device))
+    assert y.shape == (2, 3, 5) and (y == 0).all()
+    y = fp8_block_linear(torch.ones(0, device=cuda_device), torch.ones(5, 0, device=cuda_device))
+    assert y.shape == (5,) and (y == 0).all()
+
+
+def test_expert_ids_of_every_type(cuda_device):
+    """64-bit ids do not wrap into [0, E); narrow integers count; other types are refused."""
+    ex, _ = make_experts(4, 64, 48, False, 5, cuda_device)
+    x = rand(3, 64, seed=6).to(cuda_device)
+    w = torch.ones(3, 2, device=cuda_device)
+    ids = torch.tensor([[0, 3], [1, -1], [2, 4]], device=cuda_device)
+    want = fp8_expert_delta(x, ids.int(), w, ex)
+    far = ids.clone()
+    far[1, 1], far[2, 1] = 2 ** 32, -(2 ** 32) + 1
+    assert torch.equal(fp8_expert_delta(x, far, w, ex), want)
+    for dtype in (torch.int16, torch.int8):
+        assert torch.equal(fp8_expert_delta(x, ids.to(dtype), w, ex), want)
+    parts = sum(ex.delta(x, far, w, r, 2, torch.float32) for r in range(2))
+    torch.testing.assert_close(parts, want, rtol=2.0 ** -20, atol=1e-6)
+    for dtype in (torch.float32, torch.bool):
+        with pytest.raises(TypeError):
+            fp8_expert_delta(x, ids.to(dtype), w, ex)
