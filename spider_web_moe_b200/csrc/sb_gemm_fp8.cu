@@ -11,11 +11,11 @@
 //
 // Orientation: token rows are the MMA's M side (one per TMEM lane), weight rows
 // its N side (2 x 128 per tile).  An epilogue thread then holds one token row,
-// whose scale is one register, and 32 columns of each 128-row weight block,
+// whose scale is one register, and 64 columns of each 128-row weight block,
 // whose scale is another: one multiply-add per element, two at a time
 // (fma.rn.f32x2).  A SwiGLU tile holds the gate and the up rows of the same 128
 // features, so the activation and its quantisation for the next product (a
-// 1 x 128 block is the four threads of one token row) need no pass over memory
+// 1 x 128 block is the two threads of one token row) need no pass over memory
 // of their own.
 //
 // Three schedules.  One CTA per tile of 128 rows (small groups, quantised outputs);
@@ -30,6 +30,13 @@
 // which waits for the MMAs (done), finds both.  The epilogue's one arrival per
 // block (released) frees the accumulator for the MMAs two blocks on and the scale
 // slot for the scale warp four blocks on.
+//
+// What bounds the pair schedule (16384 x 4096 x 8192, 585 us, 1285 clocks a block
+// where the MMAs take 541): the epilogue's loads and additions in turn with the
+// MMAs. Without either it takes 450 us, with the loads alone 452, with the additions
+// alone 487. Accumulators in halves of 128 columns, each released by itself, took
+// 680 us (every MMA reads its rows again); 16-column loads and other orders of loads
+// and additions 580 to 600; two plain additions for a packed one 719.
 //
 // Warps: 0-7 epilogue (TMEM lane quarter w % 4, columns part w / 4), 8 TMA, 9
 // MMA (+TMEM), 10 scales.  Every wait is bounded (sb_common.cuh); loads use no
@@ -719,7 +726,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
       } else {
         // activation, then one 1 x 128 block per row (SwiGLU) or two (GELU), each
-        // held by the threads of the row in the quarter's four warps
+        // held by the threads of the row in the quarter's two warps
         constexpr int kBlocks = kGate ? 1 : 2;
         if (warp_live) {
 #pragma unroll
