@@ -566,3 +566,31 @@ def test_expert_ids_of_every_type(cuda_device):
     for dtype in (torch.float32, torch.bool):
         with pytest.raises(TypeError):
             fp8_expert_delta(x, ids.to(dtype), w, ex)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Inputs and outputs of more than 2^31 elements: the last rows are those of a small call."""
+    m, k = 70000, 32768
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda_device)
+    tail = rand(300, k, seed=1, dtype=torch.bfloat16).to(cuda_device)
+    x[-300:] = tail
+    want = quantize_fp8_blocks(tail)
+    got = quantize_fp8_blocks(x)
+    assert torch.equal(got.q[-300:].view(torch.uint8), want.q.view(torch.uint8))
+    assert torch.equal(got.scale[-300:], want.scale)
+    del got
+    cut = (m - 300) // 128 * 128  # whole blocks of 128 from here on
+    for br in (1, 128):
+        want = quantize_fp8_blocks(x[cut:].t(), br)
+        got = quantize_fp8_blocks(x.t(), br)
+        assert torch.equal(got.q[:, cut:].view(torch.uint8), want.q.view(torch.uint8))
+        assert torch.equal(got.scale[:, cut // 128:], want.scale)
+        del got
+    want = quantize_fp8_blocks(x[cut:], 128)
+    got = quantize_fp8_blocks(x, 128)
+    assert torch.equal(got.q[cut:].view(torch.uint8), want.q.view(torch.uint8))
+    assert torch.equal(got.scale[cut // 128:], want.scale)
+    del got, x
+    a, b = quantize_fp8_blocks(rand(m, 64, seed=2).to(cuda_device)), quantize_fp8_blocks(rand(k, 64, seed=3).to(cuda_device), 128)
+    last = Fp8BlockTensor(a.q[-500:], a.scale[-500:], 1)
+    assert torch.equal(F.fp8_block_matmul(a, b)[-500:], F.fp8_block_matmul(last, b))

@@ -254,3 +254,21 @@ def test_captured(cuda_device):
         graph.replay()
         want = route_experts(x.roll(i, 0), 4)
         assert torch.equal(idx, want[0]) and torch.equal(w, want[1])
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 logits: the last tokens' routing and gradient are those of a small call."""
+    n, e = 2_200_000, 1000
+    logits = torch.zeros(n, e, dtype=torch.bfloat16, device=cuda_device)
+    tail = torch.randn(257, e, generator=torch.Generator().manual_seed(1)).to(cuda_device, torch.bfloat16)
+    logits[-257:] = tail
+    grad = torch.ones(n, 4, device=cuda_device)
+    grad[:, 1] = 3.0
+    out = []
+    for x in (logits, tail):
+        x.requires_grad_()
+        idx, w = route_experts(x, 4)
+        w.backward(grad[:x.shape[0]])
+        out.append((idx[-257:], w[-257:], x.grad[-257:]))
+        assert (idx[0] == torch.arange(4, device=cuda_device)).all() or x is tail
+    assert all(torch.equal(a, b) for a, b in zip(*out))
