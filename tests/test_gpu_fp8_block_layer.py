@@ -88,3 +88,19 @@ def test_layer_captured(cuda_device):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@torch.no_grad()
+def test_layer_decode_and_statistics(cuda_device):
+    """The layer's other drivers run these experts too: early exit that never
+    exits is the loop over all blocks, and statistics do not change the output."""
+    layer, h, x0 = make("swiglu", cuda_device, torch.float32)
+    layer.quantize_experts_fp8(block_size=128)
+    want = layer.run_loops(h, x0)
+    assert torch.equal(layer.run_recurrent_decode(h, x0, early_exit=False), want)
+    h1, x1 = h[:, :1].contiguous(), x0[:, :1].contiguous()
+    got = layer.run_recurrent_decode(h1, x1, early_exit=True, threshold=2.0)
+    assert torch.equal(got, layer.run_loops(h1, x1))
+    out, stats = layer(h, x0, 0, return_stats=True)
+    assert torch.equal(out, layer(h, x0, 0)) and stats
+    check_status(cuda_device)
