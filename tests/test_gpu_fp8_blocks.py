@@ -594,3 +594,29 @@ def test_offsets_past_32_bits(cuda_device):
     a, b = quantize_fp8_blocks(rand(m, 64, seed=2).to(cuda_device)), quantize_fp8_blocks(rand(k, 64, seed=3).to(cuda_device), 128)
     last = Fp8BlockTensor(a.q[-500:], a.scale[-500:], 1)
     assert torch.equal(F.fp8_block_matmul(a, b)[-500:], F.fp8_block_matmul(last, b))
+
+
+@pytest.mark.parametrize("n", [3, 600])
+def test_gelu_of_large_values(n, cuda_device):
+    """GELU far from 0, on the decode and on the row schedule: 0 on the left, -inf
+    too; x on the right; NaN stays NaN, in the rows of its expert only."""
+    ex, _ = make_experts(2, 64, 48, False, 9, cuda_device)
+    x = rand(n, 64, seed=10).to(cuda_device)
+    idx = (torch.arange(n, device=cuda_device) % 2).view(n, 1)
+    w = torch.ones(n, 1, device=cuda_device)
+    out = {}
+    for v in (-1e4, -3e38, float("-inf"), float("nan")):
+        ex.b_up[0, 7] = v
+        out[v] = fp8_expert_delta(x, idx, w, ex)
+    a, b, c, d = out.values()
+    assert torch.isfinite(a).all() and torch.equal(a, b) and torch.equal(a, c)
+    assert torch.isnan(d[::2]).all() and torch.equal(d[1::2], a[1::2])
+    ex.b_up.fill_(0.0)
+    ex.b_up[0, 7] = 2.0 ** 20  # the block's largest: its column of w_down times 2^20, within two roundings
+    got = fp8_expert_delta(x, idx, w, ex)[::2].double()
+    ffn = x.double()[::2] @ ex.w_up.dequantize(torch.float64)[0].T
+    act = ffn[:, 7:8] + 2.0 ** 20
+    want = act * ex.w_down.dequantize(torch.float64)[0, :, 7]
+    if ex.b_down is not None:
+        want = want + ex.b_down[0].double()
+    assert ((got - want).norm(dim=1) / want.norm(dim=1)).max() < 2.0 ** -4
