@@ -350,7 +350,6 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      // the fast sigmoid is off by (1.5 |x| + 4) s (1 - s) 2^-23, below 2^-21
       c[v] = softmax ? c[v] * inv : rcp_approx(1.f + __expf(-l[v]));
     if (p.bias) {
       float b[V];
@@ -366,11 +365,16 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
   for (int v = 0; v < V; ++v)
     key[v] = lane * V + v < p.E ? (order_key(c[v]) & ~kPlaceMask<V>) | (kPlaceMask<V> - v) : 0;
   sort_descending<V>(key);
-  // fp32 error of a score: exp of a rounded difference (|x| e^-|x| 2^-24 <=
-  // 0.37 2^-24), 2 ulp of expf, the sum and the division, all below 2^-20 in all;
-  // two may differ by 2^-19.  Rounding of a choice: 2^-24 of it, and V of its
-  // last places for the expert's place.
-  constexpr float kTol = 0x1p-19f, kRel = (V + 1) * 0x1p-22f;
+  // fp32 error of scores, in u = 2^-24.  Softmax, of s: V + 4 additions of the
+  // sum, which can all round the same way, its terms (expf 4 u, and the rounded
+  // differences x: their mean under the softmax weighs at most 5), expf again, the
+  // division and the product: (V + 19) u s, and s |x| u <= 0.37 u for its own
+  // difference.  The scores of two choices, or of the four of two group scores,
+  // sum to at most 1: (V + 21) u between them.  Sigmoid: 4.6 u a score (the fast
+  // exponential 2 + 1.17 |x| ulp times s (1 - s), the addition, the reciprocal),
+  // 18.4 u for four.  Rounding of a choice: u of it, and V - 1 of its last places
+  // for the expert's place.
+  constexpr float kTol = (V + 24) * 0x1p-24f, kRel = (V + 1) * 0x1p-22f;
   // by_logit: the keys order exactly, but for the bits the place took (a bf16
   // logit has none there)
   const bool exact = by_logit && sizeof(T) == 2;
