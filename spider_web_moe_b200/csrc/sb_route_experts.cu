@@ -386,9 +386,24 @@ __global__ void __launch_bounds__(256) route_experts_kernel(const T* __restrict_
     if (p.group_top == 2 && p.per_group > 1) gs += place_key_value(k2 & ~kPlaceMask<V>);
     uint32_t gk = lane < p.groups ? order_key(gs) : 0, last;
     const uint32_t kept = best_groups(gk, p.topk_groups, lane, &last);
-    const float lc = key_value(last);
-    const uint32_t limit = by_logit ? last : order_key(lc - (2.f * kTol + 2.f * fabsf(lc) * kRel));
-    close = !exact && gk != 0 && gk >= limit;  // a group left out so close to the last one kept
+    if (by_logit) {
+      close = !exact && gk != 0 && gk >= last;  // a group left out that is the equal of the last one kept
+    } else {
+      // The error of a sum goes by its terms, not by the sum: large ones of opposite
+      // signs leave a small score known to little precision.  So the kept groups'
+      // lower ends are compared with the upper ends of those left out.  (An infinite
+      // score is exact: only infinite choices make it, or terms so large that no
+      // finite score competes.)
+      float err = 0.f;
+      if (isfinite(gs)) {
+        err = fabsf(place_key_value(k1 & ~kPlaceMask<V>));
+        if (p.group_top == 2 && p.per_group > 1) err += fabsf(place_key_value(k2 & ~kPlaceMask<V>));
+        err = 0.5f * kTol + 0.5f * kRel * err;
+      }
+      const bool group = lane < p.groups, in = group && ((kept >> lane) & 1u);
+      const uint32_t low = ~warp_max_key(in ? ~order_key(gs - err) : 0u);  // the lowest of the kept
+      close = group && !in && order_key(gs + err) >= low;
+    }
     if (p.group_shift >= 0) {
       if (!((kept >> (lane >> p.group_shift)) & 1u)) {
 #pragma unroll

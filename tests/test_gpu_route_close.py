@@ -59,3 +59,36 @@ def test_softmax_choices_around_one_value(e, cuda_device):
     s = torch.softmax(logits[0].double(), -1)
     bias = (-s * (1 + torch.randn(e, generator=g).double() * 2.0 ** -22)).float()
     check(logits.to(cuda_device), min(8, e), "softmax", bias.to(cuda_device))
+
+
+def test_group_score_of_opposite_signs(cuda_device):
+    """Group 0: 15 + 7u and -15, group 1: 15 and -15 + 3u (u = 2^-20, their last
+    place): 7u against 3u.  Order keys with the last three bits replaced read -7u
+    and +u, a gap of 7.6e-6 that a tolerance relative to the sum does not cover."""
+    u = 2.0 ** -20
+    logits = torch.zeros(1, 256)             # sigmoid: 0.5, exactly
+    bias = torch.full((256,), -1000.0)
+    bias[0], bias[1] = 14.5 + 7 * u, -15.5
+    bias[128], bias[129] = 14.5, -15.5 + 3 * u
+    kw = dict(num_groups=2, topk_groups=1)
+    idx = route_experts(logits.to(cuda_device), 1, score="sigmoid", bias=bias.to(cuda_device), **kw)[0]
+    assert definition(logits, 1, "sigmoid", bias, **kw).item() == 0 and idx.item() == 0
+
+
+@pytest.mark.parametrize("e,groups,topk_groups,size", [(1024, 32, 8, 8.0), (256, 8, 4, 16.0), (256, 8, 4, 4096.0),
+                                                       (96, 8, 2, 64.0), (480, 4, 3, 300.0), (800, 32, 9, None)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_groups_with_large_biases(e, groups, topk_groups, size, score, cuda_device):
+    """Biases of both signs, so that a group's best two choices cancel; in the last
+    case of another magnitude in each group (1 to 4096), so that the groups' scores
+    are known to different precision."""
+    g = torch.Generator().manual_seed(e + groups)
+    n, per = 60000, e // groups
+    logits = (torch.randn(n, e, generator=g) * 1.5).to(cuda_device)
+    mag = torch.full((groups, 1), size) if size else torch.exp2(torch.randint(0, 13, (groups, 1), generator=g).float())
+    bias = -mag * (1 + torch.rand(groups, per, generator=g))
+    bias[:, 0] = mag[:, 0]                   # one large positive choice and its opposite, the next best
+    bias[:, 1] = -mag[:, 0]
+    order = torch.stack([torch.randperm(per, generator=g) for _ in range(groups)])
+    bias = bias.gather(1, order).reshape(-1).contiguous().to(cuda_device)
+    check(logits, min(8, per), score, bias, num_groups=groups, topk_groups=topk_groups)
