@@ -73,7 +73,7 @@ enum {
 /* GEMM engines */
 enum { SB_ENGINE_AUTO = 0, SB_ENGINE_SIMT = 1, SB_ENGINE_TCGEN05 = 2 };
 /* grouping flags */
-enum { SB_GROUP_POSITIVE_ONLY = 1 };
+enum { SB_GROUP_POSITIVE_ONLY = 1, SB_GROUP_KEEP_NAN = 2 };
 /* expert scores of sb_route_experts */
 enum { SB_SCORE_SOFTMAX = 0, SB_SCORE_SIGMOID = 1 };
 
@@ -127,8 +127,8 @@ SB_API int sb_route_experts_backward(const void* logits, int dtype, int64_t ld, 
  * device permutation.  Entries are idx[row, slot] (row-major, `slots` per row).
  * Within a row, repeats of a group id are merged into the first occurrence and
  * their weights summed (sparse_experts.py:52-55).  With SB_GROUP_POSITIVE_ONLY
- * an entry whose summed weight is <= 0 is dropped (dispatch.py:94).  Groups
- * are laid out in ascending id, each with its rows in ascending order, so the
+ * an entry whose summed weight is <= 0 is dropped (dispatch.py:94), or NaN unless
+ * SB_GROUP_KEEP_NAN is given too.  Groups are laid out in ascending id, each with its rows in ascending order, so the
  * permutation is identical to the reference plan.
  * Outputs: offsets[G+1]; for permuted position p < offsets[G]: perm_row[p]
  * (token row), perm_slot[p] (row*slots+slot of the first occurrence),
@@ -314,7 +314,8 @@ SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t ldx, int m, 
  * e4m3 with byte pitches ld_in / ld_ffn per row (multiples of 16), scales
  * contiguous fp32 [E, ceil(rows / 128), ceil(cols / 128)], biases fp32 [E, rows]
  * or NULL.  Token rows are grouped by expert (repeated ids of a token merged,
- * weights <= 0 dropped, ids outside [0, E) skipped), quantised, and
+ * weights <= 0 dropped, ids outside [0, E) skipped; a NaN weight makes its token's
+ * delta NaN), quantised, and
  *   delta[t] = sum over t's experts of w * (down(q(act(up(q(messages[t]))))) + b_down)
  * in slot order.  messages: row pitch ld elements.  delta: [n_tokens, hidden
  * rounded up to a multiple of 4] fp32 or bf16 (the extra columns hold no

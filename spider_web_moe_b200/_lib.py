@@ -30,7 +30,7 @@ SB_W_F32, SB_W_BF16, SB_W_FP8, SB_W_INT4 = 0, 1, 2, 3
 SB_ACT_GELU, SB_ACT_SWIGLU = 0, 1
 SB_EPI_LINEAR, SB_EPI_GELU, SB_EPI_SWIGLU, SB_EPI_SWIGLU_IL = 0, 1, 2, 3
 SB_ENGINE_AUTO, SB_ENGINE_SIMT, SB_ENGINE_TCGEN05 = 0, 1, 2
-SB_GROUP_POSITIVE_ONLY = 1
+SB_GROUP_POSITIVE_ONLY, SB_GROUP_KEEP_NAN = 1, 2
 SB_SCORE_SOFTMAX, SB_SCORE_SIGMOID = 0, 1
 
 ENGINES = {"auto": SB_ENGINE_AUTO, "simt": SB_ENGINE_SIMT, "tcgen05": SB_ENGINE_TCGEN05}

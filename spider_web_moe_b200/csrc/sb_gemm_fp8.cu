@@ -1614,8 +1614,10 @@ extern "C" SB_API int sb_fp8_expert_delta(const sb_fp8_experts* experts, const v
   const int hb = (H + 127) / 128, ub = (U + 127) / 128;
   if (!status) status = b.status;
 #define SB_TRY(e) do { const int rc = (e); if (rc) return rc; } while (0)
-  SB_TRY(sb_group(top_idx, top_w, N, top_k, E, SB_GROUP_POSITIVE_ONLY, b.off, b.row, b.slot, b.w, b.inv, b.group_ws,
-                  b.group_ws_bytes, stream));
+  // NaN weights stay (the routing ranks a NaN logit first so that it is seen): they
+  // reach the token's delta as the down product's row scale
+  SB_TRY(sb_group(top_idx, top_w, N, top_k, E, SB_GROUP_POSITIVE_ONLY | SB_GROUP_KEEP_NAN, b.off, b.row, b.slot, b.w, b.inv,
+                  b.group_ws, b.group_ws_bytes, stream));
   sb_fp8_quantize_args q = {};
   q.x = messages; q.dtype = dtype; q.block_rows = 1; q.batch = 1; q.rows = P; q.cols = H;
   q.x_row = ld; q.x_col = 1; q.row_index = b.row; q.row_count = b.off + E;

@@ -14,6 +14,11 @@ namespace sb {
 
 constexpr int kGroupMaxG = 256;
 
+// Whether an entry of summed weight acc is dropped.
+SB_DEVINL bool group_drops(int flags, float acc) {
+  return (flags & SB_GROUP_POSITIVE_ONLY) && ((flags & SB_GROUP_KEEP_NAN) ? acc <= 0.f : !(acc > 0.f));
+}
+
 // Evaluate entry e = row*slots + s: returns its group (or -1) and summed weight.
 SB_DEVINL int entry_group(const int32_t* __restrict__ idx, const float* __restrict__ w, int slots,
                           int G, int flags, int64_t e, float& wsum) {
@@ -28,7 +33,7 @@ SB_DEVINL int entry_group(const int32_t* __restrict__ idx, const float* __restri
   for (int j = 0; j < slots; ++j)
     if (idx[row0 + j] == g) acc += w ? w[row0 + j] : 1.f;
   wsum = acc;
-  if ((flags & SB_GROUP_POSITIVE_ONLY) && !(acc > 0.f)) return -1;
+  if (group_drops(flags, acc)) return -1;
   return g;
 }
 
@@ -47,7 +52,7 @@ SB_DEVINL int entry_group_staged(const int32_t* s_idx, const float* s_w, int slo
   for (int j = 0; j < slots; ++j)
     if (s_idx[row0 + j] == g) acc += s_w[row0 + j];
   wsum = acc;
-  if ((flags & SB_GROUP_POSITIVE_ONLY) && !(acc > 0.f)) return -1;
+  if (group_drops(flags, acc)) return -1;
   return g;
 }
 
