@@ -407,7 +407,7 @@ template <typename T>
 static int quantize_typed(const sb_fp8_quantize_args& p, cudaStream_t st) {
   constexpr int64_t kAlign = 16 / sizeof(T);  // elements of a 16-byte load
   const bool base = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_batch % kAlign == 0;
-  if (p.block_rows == 1 && (p.x_row != 1 || p.x_col == 1 || p.row_index)) {
+  if (p.block_rows == 1 && (p.x_row != 1 || p.x_col == 1 || p.row_index || p.row_count)) {
     const dim3 grid((p.rows + kRowsPerCta - 1) / kRowsPerCta, (p.cols + 128 * kRowsBlocks - 1) / (128 * kRowsBlocks),
                     p.batch);
     if (sizeof(T) == 2 && p.x_col == 1 && base && p.x_row % 8 == 0 && p.cols % 8 == 0)
