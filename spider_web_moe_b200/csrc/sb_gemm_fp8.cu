@@ -231,22 +231,21 @@ SB_DEVINL uint64_t mul_pair(uint64_t a, uint64_t b) {
   return r;
 }
 
-// GELU for values that are quantised next: erfc(z) by Abramowitz & Stegun 7.1.28,
-// 1 / (1 + a1 z + ... + a6 z^6)^16, |error| <= 3e-7, without an exponential (64
-// experts x 256 rows x 2048 -> 1024 features: 100 -> 93 us against 7.1.26), and
-// without a difference for x < 0.  The clamp keeps infinities out of 0 * inf.
+// GELU for values that are quantised next: erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2)
+// by Abramowitz & Stegun 7.1.26 (erf_as7126's formula), |error| <= 1.5e-7, and
+// for x < 0 without a difference, so that the left tail keeps its relative
+// precision: 5e-4 of the value at x = -4 and 4e-3 at -6, where the block of a row
+// may have nothing larger.  (64 experts x 256 rows x 2048 -> 1024 features: 93 us;
+// 7.1.28, without an exponential, 87 us, but off by 4e-3 at -4 and a quarter of the
+// value at -6.)  The clamp keeps infinities out of 0 * inf.
 SB_DEVINL float gelu_fp8out(float x) {
   const float z = fabsf(x) * 0.70710678118654752f;
-  float d = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(0.0000430638f, z, 0.0002765672f), z, 0.0001520143f), z, 0.0092705272f), z,
-                           0.0422820123f), z, 0.0705230784f), z, 1.0f);
-  d *= d;
-  d *= d;
-  d *= d;
-  d *= d;
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
+  const float poly =
+      fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f) * t;
+  const float c = poly * __expf(-z * z);
   const float h = 0.5f * fminf(fmaxf(x, -1e30f), 1e30f);
-  return x > 0.0f ? fmaf(-h, r, x) : h * r;
+  return x > 0.0f ? fmaf(-h, c, x) : h * c;
 }
 
 // One item of the schedule: the rows of this CTA of one row tile of one group,
