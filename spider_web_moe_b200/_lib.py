@@ -10,6 +10,7 @@ import ctypes as C
 import os
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import build as _build
 
@@ -236,6 +237,13 @@ def ptr(t) -> int | None:
     if t is None:
         return None
     return t.data_ptr()
+
+
+def refuse_forward_ad(what: str, *tensors) -> None:
+    """The kernels read values only: a forward-mode tangent would be lost, that is
+    taken for a derivative of zero."""
+    if _fwd._current_level >= 0 and any(t is not None and _fwd.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def on_device(device, fn, *args) -> int:

@@ -138,12 +138,14 @@ def _empty_fp8(shape, device) -> torch.Tensor:
 
 def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> Fp8BlockTensor:
     """x [R, C] or [E, R, C] (float32 or bfloat16, any strides) -> Fp8BlockTensor
-    with one scale per ``block_rows`` x 128 block (block_rows 1 or 128)."""
+    with one scale per ``block_rows`` x 128 block (block_rows 1 or 128).  The values
+    have no gradient."""
     code = _dtype_code(x, "quantize_fp8_blocks input")
     if x.dim() not in (2, 3):
         raise ValueError(f"quantize_fp8_blocks needs [R, C] or [E, R, C], got shape {tuple(x.shape)}")
     if block_rows not in (1, BLOCK):
         raise ValueError(f"block_rows must be 1 or {BLOCK}, got {block_rows}")
+    L.refuse_forward_ad("quantize_fp8_blocks", x)
     _need_cuda(x, "quantize_fp8_blocks")
     x = x.detach()
     lead, (r, c) = x.shape[:-2], x.shape[-2:]
@@ -251,6 +253,7 @@ class _Fp8Linear(torch.autograd.Function):
     def backward(ctx, dy):
         if torch.is_grad_enabled():
             raise RuntimeError("fp8_block_linear is not twice differentiable")
+        L.refuse_forward_ad("fp8_block_linear", dy)
         x, weight = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         if ctx.packed is not None:
@@ -275,7 +278,7 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
     """x [..., K] (float32 or bfloat16) times weight^T -> [..., N] in x's dtype,
     in block-scaled fp8.  weight: a matrix [N, K] (float32 or bfloat16, quantised
     in the call) or an Fp8BlockTensor [N, K] packed once.  Differentiable in x
-    and in a weight matrix; all three products run in fp8.  To capture a backward
+    and in a weight matrix (once, in reverse mode); all three products run in fp8.  To capture a backward
     pass into a CUDA graph, drop eager graphs of the same leaves first: autograd
     ties their gradients to the stream those were built on."""
     packed = weight if isinstance(weight, Fp8BlockTensor) else None
@@ -289,6 +292,7 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
         raise ValueError("x and weight must be on one device")
     if packed is not None and packed.block_rows != BLOCK:
         raise ValueError("packed weights need 128 x 128 blocks")
+    L.refuse_forward_ad("fp8_block_linear", x, None if packed is not None else w)
     _need_cuda(x, "fp8_block_linear")
     flat = len(xs) == 2
     x2 = x if flat else x.reshape(xs[:-1].numel(), ws[1])
@@ -363,6 +367,7 @@ class Fp8BlockExperts:
               rank: int = 0, world: int = 1, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         """Weighted sum of the routed experts' outputs [n, H] for messages [n, H],
         experts restricted to ``e % world == rank``."""
+        L.refuse_forward_ad("fp8_expert_delta", messages, top_weights)
         lib = L.load()
         dev = self.device
         code = _dtype_code(messages, "messages")
@@ -412,6 +417,7 @@ def fp8_expert_delta(messages, top_indices, top_weights, experts: Fp8BlockExpert
     dev = experts.device
     if messages.device != dev or top_indices.device != dev or top_weights.device != dev:
         raise ValueError("messages, routing and experts must be on one device")
+    L.refuse_forward_ad("fp8_expert_delta", messages, top_weights)
     if torch.is_grad_enabled() and (messages.requires_grad or top_weights.requires_grad):
         raise NotImplementedError("fp8_expert_delta has no backward pass: call it under torch.no_grad()")
     use_ep = expert_parallel and ep_enabled()

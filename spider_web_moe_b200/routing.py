@@ -65,6 +65,7 @@ class _RouteExperts(torch.autograd.Function):
             return (None,) * 9
         if torch.is_grad_enabled():
             raise RuntimeError("route_experts is not twice differentiable")
+        L.refuse_forward_ad("route_experts", grad_w)
         logits, idx, bias = ctx.saved_tensors
         score, renormalize, scale = ctx.args
         x = _rows(logits)
@@ -93,7 +94,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     ``scale``.  An expert whose logit or bias is -inf ranks last, with weight 0.
 
     Differentiable in ``logits`` through the weights, the choice held fixed; the
-    bias has no gradient.  To capture a backward pass into a CUDA graph, drop
+    bias has no gradient; no second and no forward-mode derivatives.  To capture a backward pass into a CUDA graph, drop
     eager graphs of the same logits first: autograd ties their gradient to the
     stream those were built on.
     """
@@ -114,6 +115,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     topk_groups = num_groups if topk_groups is None else topk_groups
     if not 1 <= topk_groups <= num_groups or top_k > topk_groups * (e // num_groups):
         raise ValueError(f"topk_groups {topk_groups} of {num_groups} groups must hold top_k {top_k} experts")
+    L.refuse_forward_ad("route_experts", logits, bias)
     if bias is not None:
         if bias.shape != (e,) or bias.device != logits.device:
             raise ValueError("bias must be [E] on the logits' device")
