@@ -103,7 +103,7 @@ class SpiderMoELayer(nn.Module):
         or, with block_size 128, per 128 x 128 block (``fp8_blocks``): the experts
         then run on the fp8 tensor cores with their activations quantised too, one
         scale per row and 128 columns.  The blocks are packed at the next forward
-        pass, on its device."""
+        pass, on its device; that pass must not be under capture."""
         if block_size is not None:
             if block_size != BLOCK:
                 raise ValueError(f"block_size must be None (per output channel) or {BLOCK}, got {block_size}")
@@ -166,6 +166,9 @@ class SpiderMoELayer(nn.Module):
     def fp8_block_experts(self, device) -> Fp8BlockExperts:
         device = torch.device(device)
         if self._fp8_experts is None or self._fp8_experts.device != device:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("block-scaled experts are not packed yet: run the layer once (or "
+                                   "fp8_block_experts(device)) before capturing it")
             stack = lambda ms, j, f: torch.stack([getattr(m if j is None else m[j], f).detach() for m in ms]).to(device)  # noqa: E731
             gates = getattr(self, "expert_gates", None)
             w = lambda ms, j: stack(ms, j, "weight").float()  # noqa: E731
@@ -234,8 +237,9 @@ class SpiderMoELayer(nn.Module):
         (sb_combine_ln).  Returns (out, routing taps)."""
         rank, world = ep_helpers.get_rank_world() if use_ep else (0, 1)
         n = h.numel() // h.shape[-1]
+        experts = self.fp8_block_experts(h.device)
         msgs, top_idx, top_w = eng.route(h, loop_idx)
-        delta = self.fp8_block_experts(h.device).delta(msgs, top_idx, top_w, rank, world, torch.float32)
+        delta = experts.delta(msgs, top_idx, top_w, rank, world, torch.float32)
         if use_ep:
             ep_helpers.all_reduce_sum_(delta)
         inv = torch.arange(n, dtype=torch.int32, device=h.device).view(n, 1)
