@@ -172,9 +172,12 @@ class SpiderMoELayer(nn.Module):
             stack = lambda ms, j, f: torch.stack([getattr(m if j is None else m[j], f).detach() for m in ms]).to(device)  # noqa: E731
             gates = getattr(self, "expert_gates", None)
             w = lambda ms, j: stack(ms, j, "weight").float()  # noqa: E731
-            self._fp8_experts = Fp8BlockExperts(
+            experts = Fp8BlockExperts(
                 w(self.experts, 0), stack(self.experts, 0, "bias"), w(self.experts, 2), stack(self.experts, 2, "bias"),
                 w(gates, None) if gates is not None else None, stack(gates, None, "bias") if gates is not None else None)
+            if device.type == "cuda":  # once: the next pass may be on a stream that does not wait for this one
+                torch.cuda.current_stream(device).synchronize()
+            self._fp8_experts = experts
         return self._fp8_experts
 
     # ------------------------------------------------------------------ forward
