@@ -107,8 +107,8 @@ SB_API int sb_router(const void* h, int act_dtype, int n_tokens, int hidden, con
  * Equal choices or group scores: the smaller id first.  Decisions closer than
  * fp32 resolves are made from fp64 scores.  An expert whose logit or bias is
  * -inf ranks behind all others and has weight 0; NaN ranks first.
- * num_experts <= 1024, top_k <= 32, num_groups <= 32 and a divisor of num_experts,
- * top_k <= topk_groups * num_experts / num_groups.
+ * n_tokens <= 2^31 - 256, num_experts <= 1024, top_k <= 32, num_groups <= 32 and a
+ * divisor of num_experts, top_k <= topk_groups * num_experts / num_groups.
  *
  * sb_route_experts_backward: the gradient of top_w with respect to the logits
  * with the selection top_idx held fixed, from grad_w [n_tokens, top_k];
@@ -229,6 +229,8 @@ SB_API int sb_grouped_gemm(const sb_grouped_gemm_args* args, void* stream);
  * pitch ldq and batch stride q_batch (multiples of 16, q 16-byte aligned).  scale
  * element strides scale_row (per block of rows), scale_col, scale_batch.  The
  * bytes of q past a row's cols are not written.
+ * rows <= 2^31 - 256, but 65535 * 128 with block_rows 128 or a unit x_row (and x_col
+ * another); cols <= 2^24, batch <= 65535.
  * row_index (block_rows 1 and batch 1 only, may be NULL): row r of q is row
  * row_index[r] of x, for r < min(rows, *row_count) (device int32, may be NULL). */
 typedef struct sb_fp8_quantize_args {
@@ -263,7 +265,8 @@ SB_API int sb_fp8_quantize_blocks(const sb_fp8_quantize_args* args, void* stream
  * exponential and division; 0 below -87, where the value is under 2^-118).  bias,
  * bias_gate and row_scale may be NULL.  Output rows outside every group are
  * not written.  lda, ldb, and for quantised outputs ldo, are byte pitches and
- * multiples of 16; a, b, b_gate and a quantised out are 16-byte aligned. */
+ * multiples of 16; a, b, b_gate and a quantised out are 16-byte aligned.
+ * max_rows, n and k <= 2^31 - 256, the rows of b of all groups below 2^31. */
 typedef struct sb_fp8_matmul_args {
   int epilogue;               /* SB_EPI_LINEAR / GELU / SWIGLU */
   int out_dtype;              /* LINEAR: SB_F32 / SB_BF16 */
@@ -302,7 +305,9 @@ SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream);
  * y [m, n] contiguous, in x's dtype.
  * The backward pass: dx = dy w [m, k] (may be NULL to skip) and dw = dy^T x [n, k]
  * (may be NULL), contiguous, in x's and w's dtype; dy in x's dtype with any
- * strides; every operand quantised along the dimension its product sums over. */
+ * strides; every operand quantised along the dimension its product sums over,
+ * within the limits of sb_fp8_quantize_blocks: k <= 2^24 and n <= 65535 * 128, and
+ * for the backward pass m <= 2^24 and k <= 65535 * 128. */
 SB_API size_t sb_fp8_linear_workspace_bytes(int m, int n, int k, int packed);
 SB_API int sb_fp8_linear(const void* x, int dtype, int64_t ldx, int m, int n, int k, const void* w, int w_dtype,
                          int64_t ldw, const float* w_scale, int64_t w_scale_row, int64_t w_scale_col, void* y,
@@ -322,7 +327,7 @@ SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t ldx, int m, 
  *   delta[t] = sum over t's experts of w * (down(q(act(up(q(messages[t]))))) + b_down)
  * in slot order.  messages: row pitch ld elements.  delta: [n_tokens, hidden
  * rounded up to a multiple of 4] fp32 or bf16 (the extra columns hold no
- * values).  num_experts <= 256, top_k <= 64.  Workspace status word at offset 0
+ * values).  num_experts <= 256, top_k <= 64, n_tokens * top_k <= 2^31 - 256.  Workspace status word at offset 0
  * unless `status` is given; the workspace needs no initial contents otherwise. */
 typedef struct sb_fp8_experts {
   int num_experts, hidden, ffn;

@@ -239,6 +239,14 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+MAX_EXTENT = 2 ** 31 - 256  # the kernels' sizes are ints, rounded up to tiles
+
+
+def check_extent(what: str, size: int, limit: int = MAX_EXTENT) -> None:
+    if size > limit:
+        raise ValueError(f"{what}: at most {limit}, got {size}")
+
+
 def refuse_forward_ad(what: str, *tensors) -> None:
     """The kernels read values only: a forward-mode tangent would be lost, that is
     taken for a derivative of zero."""

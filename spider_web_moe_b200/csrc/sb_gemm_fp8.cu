@@ -1376,7 +1376,7 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
   const bool quant = a.epilogue == SB_EPI_GELU || a.epilogue == SB_EPI_SWIGLU;
   if ((!quant && a.epilogue != SB_EPI_LINEAR) || (!quant && a.out_dtype != SB_F32 && a.out_dtype != SB_BF16) ||
       a.num_groups < 1 || a.num_groups > kF8MaxG || (!a.offsets && a.num_groups != 1) || a.max_rows < 0 ||
-      a.n < 1 || a.k < 1 || (a.b_block_rows != 128 && a.b_block_rows != 1) || (quant && a.b_block_rows != 128) ||
+      a.max_rows > kMaxExtent || a.n < 1 || a.n > kMaxExtent || a.k < 1 || a.k > kMaxExtent || (a.b_block_rows != 128 && a.b_block_rows != 1) || (quant && a.b_block_rows != 128) ||
       a.lda < a.k || a.lda % 16 || a.ldb < a.k || a.ldb % 16 || (a.num_groups > 1 && a.b_group_rows < a.n) ||
       a.ldo < a.n || (quant && a.ldo % 16))
     return SB_ERR_ARG;
@@ -1456,15 +1456,18 @@ static int f8_product(const F8Buf& a, const F8Buf& b, int b_block_rows, int m, i
   g.b_block_rows = b_block_rows; g.out = out; g.ldo = n; g.status = status;
   return sb_fp8_matmul(&g, stream);
 }
+static bool f8_sizes_ok(int m, int n, int k) {
+  return m >= 0 && m <= kMaxExtent && n >= 1 && n <= kMaxExtent && k >= 1 && k <= kMaxExtent;
+}
 static bool f8_linear_ok(int dtype, int64_t ldx, int m, int n, int k, int w_dtype) {
-  return (dtype == SB_F32 || dtype == SB_BF16) && (w_dtype == SB_F32 || w_dtype == SB_BF16) && m >= 0 && n >= 1 &&
-         k >= 1 && ldx >= k;
+  return (dtype == SB_F32 || dtype == SB_BF16) && (w_dtype == SB_F32 || w_dtype == SB_BF16) && f8_sizes_ok(m, n, k) &&
+         ldx >= k;
 }
 
 }  // namespace sb
 
 extern "C" SB_API size_t sb_fp8_linear_workspace_bytes(int m, int n, int k, int packed) {
-  if (m < 0 || n < 1 || k < 1) return 0;
+  if (!f8_sizes_ok(m, n, k)) return 0;
   Carver c(nullptr, ~size_t(0) >> 1);
   f8_buf(c, m, k, 1);
   if (!packed) f8_buf(c, n, k, 128);
@@ -1497,7 +1500,7 @@ extern "C" SB_API int sb_fp8_linear(const void* x, int dtype, int64_t ldx, int m
 }
 
 extern "C" SB_API size_t sb_fp8_linear_backward_workspace_bytes(int m, int n, int k) {
-  if (m < 0 || n < 1 || k < 1) return 0;
+  if (!f8_sizes_ok(m, n, k)) return 0;
   Carver c(nullptr, ~size_t(0) >> 1);
   f8_buf(c, m, n, 1);
   f8_buf(c, k, n, 128);
@@ -1556,7 +1559,8 @@ struct F8DeltaBuffers {
 constexpr int kF8MaxExperts = 256;  // as many as sb_group takes
 
 static bool f8_experts_ok(const sb_fp8_experts* x) {
-  return x && x->num_experts >= 1 && x->num_experts <= kF8MaxExperts && x->hidden >= 1 && x->ffn >= 1 &&
+  return x && x->num_experts >= 1 && x->num_experts <= kF8MaxExperts && x->hidden >= 1 && x->hidden <= kMaxExtent &&
+         x->ffn >= 1 && x->ffn <= kMaxExtent &&
          (x->activation == SB_ACT_GELU || x->activation == SB_ACT_SWIGLU) && x->ld_in % 16 == 0 && x->ld_in >= x->hidden &&
          x->ld_ffn % 16 == 0 && x->ld_ffn >= x->ffn;
 }
@@ -1585,7 +1589,7 @@ static size_t f8_carve(const sb_fp8_experts& x, int n, int k, void* ws, size_t b
 
 extern "C" SB_API size_t sb_fp8_expert_delta_workspace_bytes(const sb_fp8_experts* experts, int n_tokens, int top_k) {
   if (!f8_experts_ok(experts) || n_tokens < 0 || top_k < 1 || top_k > 64 ||
-      static_cast<int64_t>(n_tokens) * top_k > 0x7fffffff)
+      static_cast<int64_t>(n_tokens) * top_k > kMaxExtent)
     return 0;
   F8DeltaBuffers b;
   return f8_carve(*experts, n_tokens > 0 ? n_tokens : 1, top_k, nullptr, ~size_t(0) >> 1, &b);
@@ -1597,7 +1601,7 @@ extern "C" SB_API int sb_fp8_expert_delta(const sb_fp8_experts* experts, const v
                                           size_t workspace_bytes, void* stream) {
   if (!f8_experts_ok(experts) || (dtype != SB_F32 && dtype != SB_BF16) ||
       (delta_dtype != SB_F32 && delta_dtype != SB_BF16) || n_tokens < 0 || top_k < 1 || top_k > 64 ||
-      static_cast<int64_t>(n_tokens) * top_k > 0x7fffffff || ld < experts->hidden)
+      static_cast<int64_t>(n_tokens) * top_k > kMaxExtent || ld < experts->hidden)
     return SB_ERR_ARG;
   if (n_tokens == 0) return SB_OK;
   const sb_fp8_experts& x = *experts;

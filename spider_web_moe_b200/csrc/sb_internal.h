@@ -174,6 +174,10 @@ int dequant_to_bf16(int wfmt, const void* q, const void* scales, int group_size,
 // it (sb_fp8_blocks.cu); SB_ERR_UNSUPPORTED for other matrices.
 int fp8_quantize_both(const sb_fp8_quantize_args& d, const sb_fp8_quantize_args& t, cudaStream_t st);
 
+// Largest extent of the routing and block-scaled fp8 operators: rounding one up to
+// a tile stays within an int.
+constexpr int kMaxExtent = 0x7fffff00;
+
 // Device properties cached per device.
 int current_sm_count();
 int current_cc_major();

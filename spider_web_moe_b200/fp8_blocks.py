@@ -24,6 +24,7 @@ from . import _lib as L
 from .expert_parallel import all_reduce_sum_, ep_enabled, get_rank_world
 
 BLOCK = 128
+MAX_COLS, MAX_BATCH, MAX_TILE_ROWS = 2 ** 24, 65535, 65535 * 128  # of the quantisation's grids
 _DTYPES = {torch.float32: L.SB_F32, torch.bfloat16: L.SB_BF16}
 _ID_TYPES = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
@@ -139,16 +140,21 @@ def _empty_fp8(shape, device) -> torch.Tensor:
 def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> Fp8BlockTensor:
     """x [R, C] or [E, R, C] (float32 or bfloat16, any strides) -> Fp8BlockTensor
     with one scale per ``block_rows`` x 128 block (block_rows 1 or 128).  The values
-    have no gradient."""
+    have no gradient.  At most 2^24 columns, 65535 matrices, and 65535 * 128 rows
+    (2^31 - 256 with block_rows 1, unless the rows, not the columns, are contiguous)."""
     code = _dtype_code(x, "quantize_fp8_blocks input")
     if x.dim() not in (2, 3):
         raise ValueError(f"quantize_fp8_blocks needs [R, C] or [E, R, C], got shape {tuple(x.shape)}")
     if block_rows not in (1, BLOCK):
         raise ValueError(f"block_rows must be 1 or {BLOCK}, got {block_rows}")
     L.refuse_forward_ad("quantize_fp8_blocks", x)
+    lead, (r, c) = x.shape[:-2], x.shape[-2:]
+    by_tiles = block_rows == BLOCK or (x.stride(-2) == 1 and x.stride(-1) != 1)
+    L.check_extent("rows", r, MAX_TILE_ROWS if by_tiles else L.MAX_EXTENT)
+    L.check_extent("columns", c, MAX_COLS)
+    L.check_extent("matrices", lead[0] if lead else 1, MAX_BATCH)
     _need_cuda(x, "quantize_fp8_blocks")
     x = x.detach()
-    lead, (r, c) = x.shape[:-2], x.shape[-2:]
     q = _empty_fp8(x.shape, x.device)
     cb = _blocks(c)
     if block_rows == 1:  # row-contiguous: a product reads one block's scales of many rows at a time
@@ -182,6 +188,8 @@ def fp8_block_matmul(a: Fp8BlockTensor, b: Fp8BlockTensor, out_dtype: torch.dtyp
         raise ValueError("both operands must be on one device")
     m, k = a.shape
     n = b.shape[0]
+    if max(m, n, k) > L.MAX_EXTENT:
+        raise ValueError(f"fp8_block_matmul: sizes of at most {L.MAX_EXTENT}, got {(m, n, k)}")
     if out is None:
         if out_dtype not in _DTYPES:
             raise TypeError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
@@ -277,7 +285,10 @@ class _Fp8Linear(torch.autograd.Function):
 def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
     """x [..., K] (float32 or bfloat16) times weight^T -> [..., N] in x's dtype,
     in block-scaled fp8.  weight: a matrix [N, K] (float32 or bfloat16, quantised
-    in the call) or an Fp8BlockTensor [N, K] packed once.  Differentiable in x
+    in the call) or an Fp8BlockTensor [N, K] packed once.  K <= 2^24 and N <= 65535 *
+    128 for a weight matrix; with gradients K <= 65535 * 128, and with one in the
+    weight at most 2^24 rows of x: the limits of the transposed operands' quantisation.
+    Differentiable in x
     and in a weight matrix (once, in reverse mode); all three products run in fp8.  To capture a backward
     pass into a CUDA graph, drop eager graphs of the same leaves first: autograd
     ties their gradients to the stream those were built on."""
@@ -293,10 +304,16 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
     if packed is not None and packed.block_rows != BLOCK:
         raise ValueError("packed weights need 128 x 128 blocks")
     L.refuse_forward_ad("fp8_block_linear", x, None if packed is not None else w)
-    _need_cuda(x, "fp8_block_linear")
+    grad = torch.is_grad_enabled() and (x.requires_grad or (packed is None and w.requires_grad))
     flat = len(xs) == 2
-    x2 = x if flat else x.reshape(xs[:-1].numel(), ws[1])
-    if torch.is_grad_enabled() and (x.requires_grad or (packed is None and w.requires_grad)):
+    m = xs[0] if flat else xs[:-1].numel()
+    if max(m, ws[0], ws[1]) > MAX_TILE_ROWS:
+        L.check_extent("rows of x", m, MAX_COLS if grad and packed is None and w.requires_grad else L.MAX_EXTENT)
+        L.check_extent("columns", ws[1], MAX_TILE_ROWS if grad and packed is None else MAX_COLS)
+        L.check_extent("rows of the weight", ws[0], MAX_TILE_ROWS if packed is None else MAX_COLS if grad else L.MAX_EXTENT)
+    _need_cuda(x, "fp8_block_linear")
+    x2 = x if flat else x.reshape(m, ws[1])
+    if grad:
         y = _Fp8Linear.apply(x2, None if packed is not None else w, packed)
     else:
         y = _linear(x2, w, packed)
@@ -365,14 +382,15 @@ class Fp8BlockExperts:
 
     def delta(self, messages: torch.Tensor, top_indices: torch.Tensor, top_weights: torch.Tensor,
               rank: int = 0, world: int = 1, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-        """Weighted sum of the routed experts' outputs [n, H] for messages [n, H],
-        experts restricted to ``e % world == rank``."""
+        """Weighted sum of the routed experts' outputs [n, H] for messages [n, H] and
+        top_indices / top_weights [n, K], experts restricted to ``e % world == rank``."""
         L.refuse_forward_ad("fp8_expert_delta", messages, top_weights)
-        lib = L.load()
         dev = self.device
+        n, k = top_indices.shape
+        L.check_extent("routes", n * k)
+        lib = L.load()
         code = _dtype_code(messages, "messages")
         out_dtype = messages.dtype if out_dtype is None else out_dtype
-        n, k = top_indices.shape
         x = _unit_cols(messages)
         idx, w = top_indices, top_weights
         if idx.dtype != torch.int32:

@@ -115,6 +115,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     topk_groups = num_groups if topk_groups is None else topk_groups
     if not 1 <= topk_groups <= num_groups or top_k > topk_groups * (e // num_groups):
         raise ValueError(f"topk_groups {topk_groups} of {num_groups} groups must hold top_k {top_k} experts")
+    if logits.numel() > L.MAX_EXTENT:  # else there are fewer tokens than that, too
+        L.check_extent("tokens", logits.numel() // e)
     L.refuse_forward_ad("route_experts", logits, bias)
     if bias is not None:
         if bias.shape != (e,) or bias.device != logits.device:
