@@ -288,10 +288,10 @@ def fp8_block_linear(x: torch.Tensor, weight) -> torch.Tensor:
     in the call) or an Fp8BlockTensor [N, K] packed once.  K <= 2^24 and N <= 65535 *
     128 for a weight matrix; with gradients K <= 65535 * 128, and with one in the
     weight at most 2^24 rows of x: the limits of the transposed operands' quantisation.
-    Differentiable in x
-    and in a weight matrix (once, in reverse mode); all three products run in fp8.  To capture a backward
-    pass into a CUDA graph, drop eager graphs of the same leaves first: autograd
-    ties their gradients to the stream those were built on."""
+    Differentiable in x and in a weight matrix (once, in reverse mode); all three
+    products run in fp8.  To capture a backward pass into a CUDA graph, drop eager
+    graphs of the same leaves first: autograd ties their gradients to the stream
+    those were built on."""
     packed = weight if isinstance(weight, Fp8BlockTensor) else None
     w = weight if packed is None else packed.q
     if x.dtype not in _DTYPES or (packed is None and w.dtype not in _DTYPES):
@@ -384,13 +384,28 @@ class Fp8BlockExperts:
               rank: int = 0, world: int = 1, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         """Weighted sum of the routed experts' outputs [n, H] for messages [n, H] and
         top_indices / top_weights [n, K], experts restricted to ``e % world == rank``."""
-        L.refuse_forward_ad("fp8_expert_delta", messages, top_weights)
-        dev = self.device
-        n, k = top_indices.shape
+        ks, dev = top_indices.shape, self.device
+        if len(ks) != 2 or messages.shape != (ks[0], self.hidden) or top_weights.shape != ks:
+            raise ValueError(f"need messages [n, {self.hidden}] and top_indices / top_weights [n, K], got "
+                             f"{tuple(messages.shape)}, {tuple(ks)}, {tuple(top_weights.shape)}")
+        n, k = ks
+        if not 1 <= k <= 64:
+            raise ValueError("between 1 and 64 experts per token")
         L.check_extent("routes", n * k)
-        lib = L.load()
+        if top_indices.dtype not in _ID_TYPES:
+            raise TypeError(f"top_indices must be integers, got {top_indices.dtype}")
+        if not 0 <= rank < world:
+            raise ValueError(f"rank {rank} of {world}")
+        if messages.device != dev or top_indices.device != dev or top_weights.device != dev:
+            raise ValueError("messages, routing and experts must be on one device")
+        if torch.is_grad_enabled() and (messages.requires_grad or top_weights.requires_grad):
+            raise NotImplementedError("the experts have no backward pass: call them under torch.no_grad()")
+        L.refuse_forward_ad("fp8_expert_delta", messages, top_weights)
         code = _dtype_code(messages, "messages")
         out_dtype = messages.dtype if out_dtype is None else out_dtype
+        if out_dtype not in _DTYPES:
+            raise TypeError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
+        lib = L.load()
         x = _unit_cols(messages)
         idx, w = top_indices, top_weights
         if idx.dtype != torch.int32:
@@ -428,13 +443,8 @@ def fp8_expert_delta(messages, top_indices, top_weights, experts: Fp8BlockExpert
         raise ValueError(f"need messages [..., {hidden}] and top_indices / top_weights [..., K], got {tuple(ms)}, "
                          f"{tuple(ks)}, {tuple(top_weights.shape)}")
     k = ks[-1]
-    if not 1 <= k <= 64:
+    if not 1 <= k <= 64:  # reshape below needs it too
         raise ValueError("between 1 and 64 experts per token")
-    if top_indices.dtype not in _ID_TYPES:
-        raise TypeError(f"top_indices must be integers, got {top_indices.dtype}")
-    dev = experts.device
-    if messages.device != dev or top_indices.device != dev or top_weights.device != dev:
-        raise ValueError("messages, routing and experts must be on one device")
     L.refuse_forward_ad("fp8_expert_delta", messages, top_weights)
     if torch.is_grad_enabled() and (messages.requires_grad or top_weights.requires_grad):
         raise NotImplementedError("fp8_expert_delta has no backward pass: call it under torch.no_grad()")

@@ -1,5 +1,6 @@
 """Sizes that the kernels' 32-bit arguments or grids cannot hold are refused by name,
-before any look at the device, instead of wrapping around.  Expanded tensors: no memory."""
+before any look at the device, instead of wrapping around; so are arguments of
+Fp8BlockExperts.delta that do not fit the experts.  Expanded tensors: no memory."""
 import ctypes as C
 
 import pytest
@@ -57,6 +58,22 @@ def test_product_sizes():
     for args in ((t, b), (Fp8BlockTensor(b.q, torch.ones(4, 1), 1), t)):
         with pytest.raises(ValueError, match="at most"):
             fp8_block_matmul(*args)
+
+
+@pytest.mark.parametrize("m,i,w,kw,err", [
+    ((5, 31), (5, 2), (5, 2), {}, ValueError), ((5, 32), (5, 2), (5, 3), {}, ValueError),
+    ((5, 32), (4, 2), (4, 2), {}, ValueError), ((5, 1, 32), (5, 1, 2), (5, 1, 2), {}, ValueError),
+    ((5, 32), (5, 0), (5, 0), {}, ValueError), ((5, 32), (5, 65), (5, 65), {}, ValueError),
+    ((5, 32), (5, 2), (5, 2), dict(out_dtype=torch.float16), TypeError),
+    ((5, 32), (5, 2), (5, 2), dict(rank=2, world=2), ValueError),
+])
+def test_delta_arguments(m, i, w, kw, err):
+    with pytest.raises(err):
+        Experts().delta(torch.zeros(m), torch.zeros(i, dtype=torch.int32), torch.zeros(w), **kw)
+    with pytest.raises(TypeError):
+        Experts().delta(torch.zeros(5, 32), torch.zeros(5, 2), torch.zeros(5, 2))
+    with pytest.raises(NotImplementedError):
+        Experts().delta(torch.zeros(5, 32), torch.zeros(5, 2, dtype=torch.int32), torch.zeros(5, 2, requires_grad=True))
 
 
 def test_c_abi_sizes():
