@@ -60,12 +60,15 @@ def _status_ptr(device) -> int | None:
 
 def check_status(device) -> None:
     """Raise if a kernel of this module recorded an error on ``device`` (a
-    bounded wait ran out); synchronises."""
+    bounded wait ran out); waits for all its streams."""
     device = torch.device(device)
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
     hit = _STATUS.get(device)
-    word = int(hit[0].item()) if hit is not None else 0
+    if hit is None:
+        return
+    torch.cuda.synchronize(device)
+    word = int(hit[0].item())
     if word:
         raise L.SpiderB200Error(L.SB_ERR_DEVICE_STATUS, f"fp8_blocks: device status 0x{word:x}")
 

@@ -52,3 +52,26 @@ def test_expert_parallel_pass(rank, cuda_device, monkeypatch):
     assert torch.equal(layer(h, x0, 1), want)
     assert torch.equal(F.fp8_expert_delta(msgs, idx, w, ex), alone)
     assert not torch.equal(ex.delta(msgs, idx, w, rank, 2, torch.float32), other)
+
+
+def test_status_of_another_stream(cuda_device):
+    """check_status waits for every stream of the device: an error that a kernel is
+    yet to record on another stream is seen."""
+    import spider_web_moe_b200.fp8_blocks as F
+    from spider_web_moe_b200 import _lib as L
+
+    F._status_ptr(cuda_device)
+    word = F._STATUS[cuda_device][0]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        word.fill_(4)
+    try:
+        with pytest.raises(L.SpiderB200Error, match="0x4"):
+            F.check_status(cuda_device)
+    finally:
+        side.synchronize()
+        word.zero_()
+        torch.cuda.synchronize()
+    F.check_status(cuda_device)
