@@ -1345,7 +1345,20 @@ static int launch_f8_decode(const sb_fp8_matmul_args& a, cudaStream_t st) {
 // its items of 128 x 64 fit the GPU at once: a block of k takes it about 0.45 us
 // and a 256 x 256 pair tile 0.65 us, and the same outputs are eight times the
 // items, which can then split k as well (128 x 2048 x 4096: 17.5 us in row tiles,
-// 11.8 us so).  Grouped products: by the average rows of a group.
+// 11.8 us so).
+//
+// Grouped products: by the average rows of a group, all that the host knows.  Times
+// with 16 / 32 / 64 columns / row tiles in us, 128 experts with up to two or three
+// times the average rows, SwiGLU 2048 -> 2 x 768 and LINEAR 768 -> 2048:
+//   rows  4:   68  68  73 101    41  42  46  66
+//   rows  8:   77  73  78 104    45  45  50  67
+//   rows 24:   98  87  99 105    78  60  66  72
+//   rows 32:  115  93 108 105    96  71  71  74
+//   rows 40:  136 103 110 106   112  84  76  78
+//   rows 48:  152 122 126 109   131  96  86  80  (equal groups: 140 123 116 109, 116 97 74 77)
+// GELU as SwiGLU, sooner in row tiles (rows 40: 61 / 67 / 56).  An average does not
+// see skew: 256 rows in each of 8 experts and none in 120 take 36 us in 32 columns
+// where row tiles take 23.
 static int decode_columns(const sb_fp8_matmul_args& a) {
   if (a.b_block_rows != 128) return 0;
   if (!a.offsets) {
@@ -1354,7 +1367,7 @@ static int decode_columns(const sb_fp8_matmul_args& a) {
     return a.max_rows <= 64 || items <= current_sm_count() ? 64 : 0;
   }
   const int per_group = a.max_rows / a.num_groups;
-  return per_group <= 4 ? 16 : (per_group <= 20 ? 32 : (per_group <= 48 ? 64 : 0));
+  return per_group <= 4 ? 16 : (per_group <= 32 ? 32 : (per_group <= 48 && a.epilogue == SB_EPI_LINEAR ? 64 : 0));
 }
 
 // LINEAR products: pairs pay when the rows per group fill their 256-row tiles (the

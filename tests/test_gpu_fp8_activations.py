@@ -19,7 +19,7 @@ from spider_web_moe_b200 import fp8_blocks as F
 pytestmark = pytest.mark.gpu
 
 
-def by_scale(epilogue, values, rows, device):
+def by_scale(epilogue, values, rows, device, grouped=True):
     """fp32 |gelu(v)|, or |silu(v)| with up values of 1, for every v, from every one of `rows` rows."""
     blocks, n = len(values), 128 * len(values)
     bias = torch.zeros(blocks, 128, device=device)
@@ -36,17 +36,21 @@ def by_scale(epilogue, values, rows, device):
                         a_scale=one.data_ptr(), a_scale_row=1, a_scale_block=rows, b=b.data_ptr(), ldb=128,
                         b_scale=one.data_ptr(), b_scale_row=1, b_scale_block=1, b_block_rows=128, bias=ups.data_ptr(),
                         b_gate=b.data_ptr(), b_gate_scale=one.data_ptr(), bias_gate=bias.data_ptr(),
-                        offsets=off.data_ptr(), out=out.data_ptr(), ldo=n, out_scale=scale.data_ptr(), out_scale_row=1,
+                        offsets=off.data_ptr() if grouped else None, out=out.data_ptr(), ldo=n, out_scale=scale.data_ptr(), out_scale_row=1,
                         out_scale_block=rows, status=F._status_ptr(device))
     L.check(L.load().sb_fp8_matmul(C.byref(m), torch.cuda.current_stream().cuda_stream), "sb_fp8_matmul")
     F.check_status(device)
     return scale.double().cpu() * 448
 
 
-@pytest.mark.parametrize("rows", [3, 20, 40, 200])  # decode columns of 16, 32, 64; tiles of 128 rows
-def test_gelu_values(rows, cuda_device):
+# decode columns of 16, 32, 64; tiles of 128 rows
+SCHEDULES = [(3, True), (20, True), (40, False), (200, True)]
+
+
+@pytest.mark.parametrize("rows,grouped", SCHEDULES)
+def test_gelu_values(rows, grouped, cuda_device):
     v = torch.cat([torch.linspace(-6, 6, 479), torch.tensor([-1e-3, 1e-3, 2.0 ** -20, -(2.0 ** -20), 30.0])])
-    got = by_scale(L.SB_EPI_GELU, v, rows, cuda_device)
+    got = by_scale(L.SB_EPI_GELU, v, rows, cuda_device, grouped)
     x = v.double()
     want = (0.5 * x * torch.special.erfc(-x * 0.5 ** 0.5)).abs()[:, None]
     tol = 1.5e-7 * 0.5 * x.abs()[:, None] + 2.0 ** -18 * want + 2.0 ** -100
@@ -54,10 +58,10 @@ def test_gelu_values(rows, cuda_device):
     assert (err <= tol).all(), [(float(v[i]), float((err / want)[i].max())) for i in (err > tol).any(1).nonzero().flatten()][:8]
 
 
-@pytest.mark.parametrize("rows", [3, 20, 40, 200])
-def test_silu_values(rows, cuda_device):
+@pytest.mark.parametrize("rows,grouped", SCHEDULES)
+def test_silu_values(rows, grouped, cuda_device):
     v = torch.cat([torch.linspace(-60, 60, 479), torch.tensor([-1e-3, 1e-3, 2.0 ** -20, -(2.0 ** -20), -86.0, -1e4, 1e4])])
-    got = by_scale(L.SB_EPI_SWIGLU, v, rows, cuda_device)
+    got = by_scale(L.SB_EPI_SWIGLU, v, rows, cuda_device, grouped)
     x = v.double()
     want = (x * torch.sigmoid(x)).abs().clamp_min(2.0 ** -100)[:, None]  # the format's floor of a block's amax
     tol = (6 + 1.2 * x.abs()[:, None]) * 2.0 ** -23 * want + 2.0 ** -100
