@@ -26,10 +26,10 @@
 //
 // Scales come through shared memory from a warp of their own, which works up to
 // four blocks ahead: it loads a block's scales, multiplies them, writes them to
-// one of four slots and arrives on the slot's barrier (scaled), for which the
-// epilogue waits beside the MMAs' (done).  The epilogue's one arrival per block
-// (released) frees the accumulator for the MMAs two blocks on and the scale slot
-// for the scale warp four blocks on.
+// one of four slots and arrives on the block's barrier (done) beside the MMAs'
+// commit, so that the epilogue's one wait finds both.  The epilogue's one arrival
+// per block (released) frees the accumulator for the MMAs two blocks on and the
+// scale slot for the scale warp four blocks on.
 //
 // What bounds the pair schedule (16384 x 4096 x 8192, 585 us, 1285 clocks a block
 // where the MMAs take 541): the epilogue's loads and additions in turn with the
@@ -76,7 +76,7 @@ struct F8Cfg {
   static constexpr int kBoxBytes = 32 * 128;
   static constexpr int kOffOut = kOffB + kStages * kBBytes;
   static constexpr int kOffBar = kOffOut + (kPair ? kEpiWarps * 2 * kBoxBytes : 0);
-  static constexpr int kOffMisc = kOffBar + (2 * kStages + 8) * 8;
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + 4) * 8;
   static constexpr int kOffMax = (kOffMisc + 64 + 15) / 16 * 16;                            // uint32 [2 blocks][kParts][128 rows]
   // What the epilogue needs once per item, from the scale warp: bias of the tile's
   // 256 columns, row scale of its 128 rows.  The scale warp is at most four blocks,
@@ -90,6 +90,7 @@ struct F8Cfg {
   static constexpr int kSmemBytes = kOffOffsets + (kF8MaxG + 1) * 4 + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(kTmemCols == 512, "two accumulators of 256 columns");
+  static_assert(kStages == 4, "a block's stage and its scale slot have one number");
   static_assert(kOffItem % 16 == 0 && kOffScale % 16 == 0, "16-byte reads");
 };
 
@@ -323,16 +324,15 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // a pair uses the leader's
-  // A block's MMAs are done: its stage is free and its accumulator is complete.
-  // (The MMAs of the stage's next use wait until every warp has waited for this one.)
+  // A block's MMAs are done and its scales (with an item's first block its bias and
+  // row scales) are written: the commit and this CTA's scale warp arrive.  The
+  // warp's own arrival orders its stores before the epilogue's reads, which a commit,
+  // in a pair the other CTA's, would not.  The stage is free, too.  (The MMAs and the
+  // scales of the stage's next use wait until every warp has waited for this one.)
   uint64_t* done = full + S;
   // [4], by block: the epilogue has read the accumulator and the scales.  The
   // leader's of a pair counts both CTAs' warps.
   uint64_t* released = done + S;
-  // [4], by block: this CTA's scale warp has written the block's scales (and with an
-  // item's first block its bias and row scales).  The epilogue waits for it beside
-  // `done`: a commit orders the tensor core's accesses, not another warp's stores.
-  uint64_t* scaled = released + 4;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
@@ -348,12 +348,9 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&done[s], 1);
+      mbar_init(&done[s], 2);  // the commit, and this CTA's scale warp
     }
-    for (int b = 0; b < 4; ++b) {
-      mbar_init(&released[b], C::kEpiWarps * (kPair && rank == 0 ? 2 : 1));
-      mbar_init(&scaled[b], 1);
-    }
+    for (int b = 0; b < 4; ++b) mbar_init(&released[b], C::kEpiWarps * (kPair && rank == 0 ? 2 : 1));
     fence_barrier_init();
   }
   if (warp == kTmaWarp && lane == 0) {
@@ -553,7 +550,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               for (int j = 0; j < kB; ++j) f[C::kBM + lane + 32 * j] = sb[i][j];
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&scaled[rel.slot]);
+            if (lane == 0) mbar_arrive(&done[rel.slot]);  // S == 4: the block's stage
             rel.next();
             load(kk0 + i + kAhead, i);
           }
@@ -590,8 +587,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
       for (int kk = 0; kk < nk; ++kk, ++it) {
         const uint32_t slot = it & 3;
-        if (!__all_sync(0xffffffffu, mbar_wait(&scaled[slot], (it >> 2) & 1, p.status, SB_DEVERR_EPI_WAIT) &&
-                                         mbar_wait(&done[slot], (it >> 2) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&done[slot], (it >> 2) & 1, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
@@ -855,7 +851,7 @@ struct F8DecCfg {
   static constexpr int kCols = kN / 2;  // columns per epilogue thread and tile
   static constexpr int kOffX = kStages * kTiles * kWBytes;
   static constexpr int kOffBar = kOffX + kStages * kXBytes;
-  static constexpr int kOffMisc = kOffBar + (2 * kStages + 2 * kAcc) * 8;
+  static constexpr int kOffMisc = kOffBar + (2 * kStages + kAcc) * 8;
   static constexpr int kOffScale = (kOffMisc + 16 + 15) / 16 * 16;         // float [kAcc][kTiles][kN]
   static constexpr int kOffMax = kOffScale + kAcc * kTiles * kN * 4;       // uint32 [kN][4 quarters]
   static constexpr int kOffPrefix = kOffMax + kN * 4 * 4;
@@ -921,9 +917,8 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* done = full + S;  // stage free and accumulator complete (S >= kAcc)
+  uint64_t* done = full + S;  // stage free, accumulator complete (S >= kAcc), scales written: as above
   uint64_t* acc_empty = done + S;
-  uint64_t* scaled = acc_empty + C::kAcc;  // the scale warp's stores, for the epilogue
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   int* s_off = reinterpret_cast<int*>(smem + C::kOffOffsets);
@@ -940,12 +935,9 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 2);  // the copies, and the scale warp
-      mbar_init(&done[s], 1);
+      mbar_init(&done[s], 2);  // the commit, and the scale warp
     }
-    for (int b = 0; b < C::kAcc; ++b) {
-      mbar_init(&acc_empty[b], 8);
-      mbar_init(&scaled[b], 1);
-    }
+    for (int b = 0; b < C::kAcc; ++b) mbar_init(&acc_empty[b], 8);
     fence_barrier_init();
   }
   if (warp == 8 && lane == 0) {
@@ -1077,7 +1069,7 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             }
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&scaled[acc.slot]);
+            mbar_arrive(&done[st.slot]);
             mbar_arrive(&full[st.slot]);  // passes the free accumulator on to the MMAs
           }
           st.next();
@@ -1112,8 +1104,7 @@ f8_decode_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         for (int i = 0; i < NC / 2; ++i) sum[h][i] = 0;
       for (int kk = 0; kk < nk; ++kk, st.next(), ring_acc.next()) {
         const int buf = ring_acc.slot;
-        if (!__all_sync(0xffffffffu, mbar_wait(&scaled[buf], ring_acc.parity, p.status, SB_DEVERR_EPI_WAIT) &&
-                                         mbar_wait(&done[st.slot], st.parity, p.status, SB_DEVERR_EPI_WAIT))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&done[st.slot], st.parity, p.status, SB_DEVERR_EPI_WAIT))) {
           ok = false;
           break;
         }
