@@ -254,7 +254,8 @@ SB_API int sb_fp8_quantize_blocks(const sb_fp8_quantize_args* args, void* stream
  * offsets NULL with num_groups 1: all rows)
  *   acc[r, c] = sum_kb a_scale[r, kb] * b_scale[c / b_block_rows, kb] *
  *               sum_{k in block kb} a[r, k] * b_g[c, k]
- * with the inner sums and the running sum in fp32, then the epilogue:
+ * with the inner sums and the running sum in fp32 (24 bits; the tensor core rounds
+ * the inner ones towards zero), then the epilogue:
  *   SB_EPI_LINEAR  out[r, c] = (acc + bias_g[c]) * row_scale[r], fp32 or bf16
  *   SB_EPI_GELU    out = gelu_erf(acc + bias_g[c])
  *   SB_EPI_SWIGLU  out = silu(acc_gate + bias_gate_g[c]) * (acc + bias_g[c])

@@ -31,12 +31,16 @@
 // per block (released) frees the accumulator for the MMAs two blocks on and the
 // scale slot for the scale warp four blocks on.
 //
-// What bounds the pair schedule (16384 x 4096 x 8192, 585 us, 1285 clocks a block
-// where the MMAs take 541): the epilogue's loads and additions in turn with the
-// MMAs. Without either it takes 450 us, with the loads alone 452, with the additions
-// alone 487. Accumulators in halves of 128 columns, each released by itself, took
-// 680 us (every MMA reads its rows again); 16-column loads and other orders of loads
-// and additions 580 to 600; two plain additions for a packed one 719.
+// What bounds the pair schedule (16384 x 4096 x 8192, 576 to 594 us on different
+// GPUs, about 1300 clocks a block of k where its MMAs take 541).  Measured at 594 us:
+// without the additions 448, without the TMEM loads 487, without either 455.  So
+// loads and additions account for 300 of the 760 clocks above the MMAs; the other
+// 460 are the hand-overs between the roles (commit to wait, release to issue,
+// operands arriving), which these times do not split further.  Accumulators in
+// halves of 128 columns, each released by itself, took 680 us (every MMA reads its
+// rows again); 16-column loads and other orders of loads and additions 580 to 600;
+// two plain additions for a packed one 719; the scales' barrier waited for by itself
+// 596 (576 as it is).
 //
 // Warps: 0-7 epilogue (TMEM lane quarter w % 4, columns part w / 4), 8 TMA, 9
 // MMA (+TMEM), 10 scales.  Every wait is bounded (sb_common.cuh); loads use no
@@ -66,7 +70,8 @@ struct F8Cfg {
   static constexpr int kEpiWarps = 4 * kParts;
   static constexpr int kThreads = (kEpiWarps + 4) * 32;  // whole warpgroups: registers move between them
   // Registers per thread at launch (65536 / kThreads, in steps of 8) and after
-  // the split.
+  // the split.  The compiler spills in all of these kernels: 34 bytes a thread in the
+  // pair's, 90 to 160 in most, 310 with GELU.
   static constexpr int kRegsLaunch = 168, kRegsEpi = 224, kRegsLoad = 56;
   static_assert(kEpiWarps * 32 * kRegsEpi + 128 * kRegsLoad <= kThreads * kRegsLaunch, "the split must fit the launch's registers");
   static constexpr int kSmallRows = 32;                // rows of the box that short tiles load
@@ -186,10 +191,12 @@ SB_DEVINL void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[kN / 2]) {
 #pragma unroll
   for (int i = 0; i < kN / 2; ++i) asm("mov.b64 %0, {%1, %2};" : "=l"(v[i]) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
 }
-// Arrive on a barrier of the pair's leader.  What it hands over is an accumulator,
+// Arrive on a barrier of the pair's leader.  What it hands over is an accumulator and
+// nothing else (scales and their slots stay within a CTA and its own barriers),
 // ordered by the tcgen05 fences on both sides, so the default CTA-scope release
 // does: a cluster-scope one waits for every outstanding access of the thread,
-// once per block of k (16384 x 4096 x 8192: 1190 us with it, 685 us without).
+// once per block of k (16384 x 4096 x 8192: 1190 us with it, 685 us without, in a
+// form of the kernel that took 685).
 SB_DEVINL void mbar_arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
