@@ -128,8 +128,8 @@ SB_API int sb_route_experts_backward(const void* logits, int dtype, int64_t ld, 
  * Within a row, repeats of a group id are merged into the first occurrence and
  * their weights summed (sparse_experts.py:52-55).  With SB_GROUP_POSITIVE_ONLY
  * an entry whose summed weight is <= 0 is dropped (dispatch.py:94), or NaN unless
- * SB_GROUP_KEEP_NAN is given too.  Groups are laid out in ascending id, each with its rows in ascending order, so the
- * permutation is identical to the reference plan.
+ * SB_GROUP_KEEP_NAN is given too.  Groups are laid out in ascending id, each with
+ * its rows in ascending order, so the permutation is identical to the reference plan.
  * Outputs: offsets[G+1]; for permuted position p < offsets[G]: perm_row[p]
  * (token row), perm_slot[p] (row*slots+slot of the first occurrence),
  * perm_w[p] (summed weight; w may be NULL -> 1); inv[row*slots+slot] = p or -1.
@@ -328,8 +328,9 @@ SB_API int sb_fp8_linear_backward(const void* x, int dtype, int64_t ldx, int m, 
  *   delta[t] = sum over t's experts of w * (down(q(act(up(q(messages[t]))))) + b_down)
  * in slot order.  messages: row pitch ld elements.  delta: [n_tokens, hidden
  * rounded up to a multiple of 4] fp32 or bf16 (the extra columns hold no
- * values).  num_experts <= 256, top_k <= 64, n_tokens * top_k <= 2^31 - 256.  Workspace status word at offset 0
- * unless `status` is given; the workspace needs no initial contents otherwise. */
+ * values).  num_experts <= 256, top_k <= 64, n_tokens * top_k <= 2^31 - 256.
+ * Workspace status word at offset 0 unless `status` is given; the workspace needs
+ * no initial contents otherwise. */
 typedef struct sb_fp8_experts {
   int num_experts, hidden, ffn;
   int activation; /* SB_ACT_GELU / SB_ACT_SWIGLU */

@@ -446,7 +446,8 @@ extern "C" SB_API int sb_fp8_quantize_blocks(const sb_fp8_quantize_args* args, v
   if (!args) return SB_ERR_ARG;
   const sb_fp8_quantize_args& p = *args;
   if ((p.dtype != SB_F32 && p.dtype != SB_BF16) || (p.block_rows != 1 && p.block_rows != 128) || p.batch < 0 ||
-      p.batch > 65535 || p.rows < 0 || p.rows > kMaxExtent || p.cols < 0 || p.cols > kMaxCols || p.ldq % 16 || p.q_batch % 16 || p.ldq < p.cols ||
+      p.batch > 65535 || p.rows < 0 || p.rows > kMaxExtent || p.cols < 0 || p.cols > kMaxCols ||
+      p.ldq % 16 || p.q_batch % 16 || p.ldq < p.cols ||
       ((p.row_index || p.row_count) && (p.block_rows != 1 || p.batch != 1)))
     return SB_ERR_ARG;
   if (p.batch == 0 || p.rows == 0 || p.cols == 0) return SB_OK;

@@ -1387,7 +1387,8 @@ extern "C" SB_API int sb_fp8_matmul(const sb_fp8_matmul_args* args, void* stream
   const bool quant = a.epilogue == SB_EPI_GELU || a.epilogue == SB_EPI_SWIGLU;
   if ((!quant && a.epilogue != SB_EPI_LINEAR) || (!quant && a.out_dtype != SB_F32 && a.out_dtype != SB_BF16) ||
       a.num_groups < 1 || a.num_groups > kF8MaxG || (!a.offsets && a.num_groups != 1) || a.max_rows < 0 ||
-      a.max_rows > kMaxExtent || a.n < 1 || a.n > kMaxExtent || a.k < 1 || a.k > kMaxExtent || (a.b_block_rows != 128 && a.b_block_rows != 1) || (quant && a.b_block_rows != 128) ||
+      a.max_rows > kMaxExtent || a.n < 1 || a.n > kMaxExtent || a.k < 1 || a.k > kMaxExtent ||
+      (a.b_block_rows != 128 && a.b_block_rows != 1) || (quant && a.b_block_rows != 128) ||
       a.lda < a.k || a.lda % 16 || a.ldb < a.k || a.ldb % 16 || (a.num_groups > 1 && a.b_group_rows < a.n) ||
       a.ldo < a.n || (quant && a.ldo % 16))
     return SB_ERR_ARG;
@@ -1630,8 +1631,8 @@ extern "C" SB_API int sb_fp8_expert_delta(const sb_fp8_experts* experts, const v
 #define SB_TRY(e) do { const int rc = (e); if (rc) return rc; } while (0)
   // NaN weights stay (the routing ranks a NaN logit first so that it is seen): they
   // reach the token's delta as the down product's row scale
-  SB_TRY(sb_group(top_idx, top_w, N, top_k, E, SB_GROUP_POSITIVE_ONLY | SB_GROUP_KEEP_NAN, b.off, b.row, b.slot, b.w, b.inv,
-                  b.group_ws, b.group_ws_bytes, stream));
+  SB_TRY(sb_group(top_idx, top_w, N, top_k, E, SB_GROUP_POSITIVE_ONLY | SB_GROUP_KEEP_NAN, b.off, b.row, b.slot, b.w,
+                  b.inv, b.group_ws, b.group_ws_bytes, stream));
   sb_fp8_quantize_args q = {};
   q.x = messages; q.dtype = dtype; q.block_rows = 1; q.batch = 1; q.rows = P; q.cols = H;
   q.x_row = ld; q.x_col = 1; q.row_index = b.row; q.row_count = b.off + E;

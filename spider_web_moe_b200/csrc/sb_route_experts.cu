@@ -564,8 +564,8 @@ route_experts_backward_kernel(const T* __restrict__ logits, const __grid_constan
 }
 
 static bool route_args_ok(int dtype, int64_t ld, int n, int E, int K, int score) {
-  return (dtype == SB_F32 || dtype == SB_BF16) && n >= 0 && n <= kMaxExtent && E > 0 && E <= kRouteMaxE && K > 0 && K <= E &&
-         K <= kRouteMaxK && ld >= E && (score == SB_SCORE_SOFTMAX || score == SB_SCORE_SIGMOID);
+  return (dtype == SB_F32 || dtype == SB_BF16) && n >= 0 && n <= kMaxExtent && E > 0 && E <= kRouteMaxE && K > 0 &&
+         K <= E && K <= kRouteMaxK && ld >= E && (score == SB_SCORE_SOFTMAX || score == SB_SCORE_SIGMOID);
 }
 
 static int route_warps(int E) { return E <= 256 ? 8 : 4; }

@@ -439,8 +439,9 @@ def fp8_expert_delta(messages, top_indices, top_weights, experts: Fp8BlockExpert
     """``sparse_expert_delta`` with block-scaled fp8 experts: messages [..., H]
     (float32 or bfloat16), top_indices / top_weights [..., K] -> delta [..., H] in
     the messages' dtype.  Repeated ids of a token add their weights, weights <= 0
-    and ids outside [0, E) are skipped, a NaN weight makes its token's delta NaN; under expert parallelism each rank runs
-    its own experts and the delta is summed across ranks.  Inference only."""
+    and ids outside [0, E) are skipped, a NaN weight makes its token's delta NaN;
+    under expert parallelism each rank runs its own experts and the delta is summed
+    across ranks.  Inference only."""
     ms, ks, hidden = messages.shape, top_indices.shape, experts.hidden
     if not ms or ms[-1] != hidden or ks != top_weights.shape or ks[:-1] != ms[:-1]:
         raise ValueError(f"need messages [..., {hidden}] and top_indices / top_weights [..., K], got {tuple(ms)}, "
