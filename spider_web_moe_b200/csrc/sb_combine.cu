@@ -466,9 +466,12 @@ combine_ln_wait_warp_kernel(const float* __restrict__ y, int64_t ldy, const int3
 using namespace sb;
 
 namespace {
-// Warp-per-token variants for large batches (from 512 tokens): cols a
-// multiple of 128 up to 2048 (NV float4 chunks per lane).
-bool use_warp_rows(int n_tokens, int cols) { return n_tokens >= 512 && cols % 128 == 0 && cols <= 2048; }
+// Warp-per-token variants for large batches (from 512 tokens): cols 128, 256, 512,
+// 1024 or 2048 (NV float4 chunks per lane, the cases of the switches below); other
+// widths take a CTA per token at any batch.
+bool use_warp_rows(int n_tokens, int cols) {
+  return n_tokens >= 512 && cols % 128 == 0 && cols <= 2048 && (cols & (cols - 1)) == 0;
+}
 
 template <typename T>
 int launch_combine_rows_warp(const float* y, int64_t ldy, int splits, int64_t split_stride, const int32_t* inv,
