@@ -681,9 +681,11 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       if constexpr (!kQuant) {
         if (!ok || !warp_live) continue;
         const float rs = s_bias[2 * C::kHalf - part * NC + r];
-        // whole boxes of 32 rows leave through shared memory (the hardware clips
-        // columns past n); element stores would keep the warp, and with it the
-        // tensor core, waiting for 16-byte pieces of 32 different rows
+        // whole boxes of 32 rows leave through shared memory; element stores would keep
+        // the warp, and with it the tensor core, waiting for 16-byte pieces of 32
+        // different rows.  The hardware clips a box at n, but in units of 16 bytes:
+        // where n is no multiple of that (tma_out 1), a box that holds the end is
+        // stored by element, or zeros would land behind the row
         const bool staged = kPair && tma_out && quarter * 32 + 32 <= w.rows;
         uint8_t* box = smem + C::kOffOut + warp * 2 * C::kBoxBytes;
         if (staged) {
@@ -707,7 +709,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < NC; ++i) acc[h][i] *= rs;
           }
-          if (staged) {
+          if (staged && (valid >= NC || tma_out > 1)) {
             if (p.out_dtype == SB_F32) {
               if (h == 1) {
                 if (lane == 0) tma_store_wait_read();
@@ -1277,10 +1279,11 @@ static int launch_f8(const sb_fp8_matmul_args& a, cudaStream_t st) {
   // bytes; without one (an unaligned output) every element is stored by its thread
   CUtensorMap mo = ma;
   const int esize = a.out_dtype == SB_F32 ? 4 : 2;
-  const int tma_out =
+  const bool boxes =
       kPair && EPI == SB_EPI_LINEAR && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * esize % 16 == 0 &&
       make_map(&mo, a.out, esize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n,
                a.max_rows, a.ldo * esize, 128 / esize, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  const int tma_out = boxes ? (static_cast<int64_t>(a.n) * esize % 16 == 0 ? 2 : 1) : 0;  // 2: the end of a row, too
   const int64_t n_tiles = (a.n + kTileCols - 1) / kTileCols;
   const int64_t row_tiles = (a.max_rows + C::kItemRows - 1) / C::kItemRows + (a.offsets ? a.num_groups : 0);
   if (n_tiles * row_tiles > 0x7fffffff) return SB_ERR_UNSUPPORTED;
